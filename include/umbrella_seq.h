@@ -669,6 +669,37 @@ int umb_lat_attend_tiled_ok(int H, int kv_rank, int rot_dim, int dtype);
 
 int umb_seq_forward(const UmbSeqModel* m, const UmbSeqWork* ws, const UmbSeqStep* s, umb_stream_t stream);
 
+/* ------------------------------------------------------------------ steps of many requests at once */
+
+/* The next token of every row of logits (fp32, rows ld apart), each with its own settings: fp32 temperature [rows], int32 top_k, fp32 top_p and min_p
+ * (null: 1, all, 1, 0), and a given random number uniforms [rows].  Order: value descending, index ascending; w = exp((x - max) / T).  Kept is the shortest
+ * of three prefixes of that order: the first top_k (<= 0 or >= V: all); those in front of which less than top_p of the first top_k's mass stands (top_p >= 1 or
+ * NaN: all; at least the first); those with w >= min_p (at least the first).  Drawn is the first kept token whose mass with all in front of it exceeds u times
+ * the kept mass; u is taken into [0, 1).  T <= 0 or NaN: the first token.  -inf and NaN are never drawn; a row of nothing else gives -1.  Largest values that
+ * are infinite share all mass.  tokens [rows]; probs [rows] (may be null): the drawn token's share of the kept mass (1 where T <= 0, 0 beside -1).
+ * V <= 524288.  scratch: umb_sample_requests_bytes(rows, V) bytes (no stream), 16-byte aligned, anything in it; nothing is kept there between calls. */
+long umb_sample_requests_bytes(int rows, int V);
+int umb_sample_requests(int* tokens, float* probs, const float* logits, long ld, int rows, int V, const float* uniforms, const float* temperature,
+                        const int* top_k, const float* top_p, const float* min_p, void* scratch, long scratch_bytes, umb_stream_t stream);
+
+/* Pages copied from place to place, in every pool of a cache.  A pool: an array of pages of page_bytes at address `base`, each [groups][rows][row_bytes] at its
+ * front; `per`: the tokens that a row stands for (1: keys, values, latents; a pooled block's length; 0: pages move whole, a recurrent layer's slots).
+ * moves int32 [n_moves][3] = {src, dst, tokens}: the first ceil(tokens / per) rows of each group of dst become src's, the others stay.  No dst is another move's
+ * dst or src.  A move with a page outside 0 .. n_pages - 1, of a page to itself or of no tokens does nothing.
+ * table (may be null): int32 [n_table] page numbers p, those in 0 .. n_pages - 1 replaced by where[p] (int32 [n_pages]).
+ * `pools` is host memory, read during the call. */
+typedef struct UmbPagePool { int64_t base, page_bytes, groups, rows, row_bytes, per; } UmbPagePool;
+int umb_pages_copy(const UmbPagePool* pools, int n_pools, const int* moves, int n_moves, int n_pages, int* table, long n_table, const int* where,
+                   umb_stream_t stream);
+
+/* Low-rank adapters of many requests beside a shared product: out[t] = base[t] + scale[a] B_a (A_a x[t]), a = adapter[t]; a outside 0 .. S - 1: base[t].
+ * out and base fp32 [T][N] (may be the same); x [T][K], A [S][R][K], B [S][N][R] in `dtype`; adapter int32 [T]; scale fp32 [S] (null: 1), rank int32 [S]
+ * (null: R): of adapter a's R rows of A and columns of B the first rank[a] count, whatever stands in the others.  R <= 128.
+ * scratch: umb_seq_adapters_parts(T, K) T R floats (no stream). */
+int umb_seq_adapters_parts(int T, int K);
+int umb_seq_adapters(float* out, const float* base, const void* x, const void* a, const void* b, const int* adapter, const float* scale, const int* rank, int T,
+                     int N, int K, int S, int R, float* scratch, long scratch_floats, int dtype, umb_stream_t stream);
+
 /* sampling on fp32 logits rows (the same kernels as libumbrella_hip.so) */
 int umb_argmax_rows(int* out, const float* logits, int rows, int V, umb_stream_t stream);
 int umb_sample_rows(int* sampled, float* logits, int rows, int V, const int* tokens_all, const int* n_ptr,

@@ -391,9 +391,14 @@ SEQ_SIGNATURES = {
     "umb_seq_forward": [C.POINTER(UmbSeqModel), C.POINTER(UmbSeqWork), C.POINTER(UmbSeqStep)],
     "umb_argmax_rows": [_P, _P, _I, _I],
     "umb_sample_rows": [_P, _P, _I, _I, _P, _P, _F, _F, _I, _F, _P, _I, _P, _P],
+    "umb_sample_requests_bytes": [_I, _I],
+    "umb_sample_requests": [_P, _P, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _L],
+    "umb_pages_copy": [_P, _I, _P, _I, _I, _P, _L, _P],
+    "umb_seq_adapters_parts": [_I, _I],
+    "umb_seq_adapters": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _L, _I],
     "umb_seq_version": [],
 }
-_SEQ_NO_STREAM = {"umb_lat_attend_tiled_ok", "umb_seq_front_ok", "umb_seq_linear_split", "umb_seq_tile_kind", "umb_seq_tile_mix", "umb_lin_scan_columns", "umb_seq_resid_canon_step_ok", "umb_bsa_attend_tiled_ok", "umb_mingru_scratch_floats",
+_SEQ_NO_STREAM = {"umb_sample_requests_bytes", "umb_seq_adapters_parts", "umb_lat_attend_tiled_ok", "umb_seq_front_ok", "umb_seq_linear_split", "umb_seq_tile_kind", "umb_seq_tile_mix", "umb_lin_scan_columns", "umb_seq_resid_canon_step_ok", "umb_bsa_attend_tiled_ok", "umb_mingru_scratch_floats",
                   "umb_ssd_scan_chunked_floats", "umb_delta_scan_floats", "umb_gla_scan_chunked_floats"}          # predicates: no stream argument, the value is the answer
 _seq_lib = None
 
@@ -413,7 +418,7 @@ def load_seq() -> C.CDLL:
         if name == "umb_seq_version":
             fn.argtypes, fn.restype = [], C.c_char_p
         elif name in _SEQ_NO_STREAM:
-            fn.argtypes, fn.restype = list(args), (C.c_long if name.endswith("_floats") else C.c_int)
+            fn.argtypes, fn.restype = list(args), (C.c_long if name.endswith(("_floats", "_bytes")) else C.c_int)
         else:
             fn.argtypes, fn.restype = list(args) + [_P], C.c_int
     _seq_lib = lib
@@ -434,6 +439,14 @@ def seq_call(name: str, *args):
     rc = getattr(lib, name)(*conv, stream_ptr())
     if rc != 0:
         raise UmbError(f"libumbrella_seq {name} failed with code {rc}")
+
+
+def seq_call_on(device, name: str, *args):
+    """seq_call on the current stream of `device`, whichever device is the current one"""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return seq_call(name, *args)
+    with torch.cuda.device(device):
+        return seq_call(name, *args)
 
 
 _lib = None

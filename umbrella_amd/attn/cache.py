@@ -149,6 +149,26 @@ def send(host: torch.Tensor, device, into: torch.Tensor = None) -> torch.Tensor:
     return host.to(device, non_blocking=True) if into is None else into.copy_(host, non_blocking=True)
 
 
+def copy_pages(pools, moves, n_pages: int, table=None, where=None):
+    """Copies pages in every pool of a cache by one launch (include/umbrella_seq.h, ``umb_pages_copy``).
+
+    pools: int64 ``[n, 6]`` on the host, a row per pool: address, bytes a page, groups, rows, bytes a row, tokens a row stands for (0: pages
+    move whole); moves: int32 ``[n, 3]`` on the device, (src, dst, tokens): the first rows, up to `tokens`, of every group of page dst become
+    src's.  No dst is another move's dst or src.  With `table` (int32, any shape) and `where` (int32 ``[n_pages]``) every page number p of the
+    table is replaced by where[p]."""
+    if pools.device.type != "cpu" or pools.dtype != torch.int64 or pools.dim() != 2 or pools.shape[1] != 6 or not pools.is_contiguous():
+        raise ValueError(f"pools: a contiguous int64 [n, 6] tensor on the host is wanted, got {pools.dtype} {tuple(pools.shape)} on {pools.device}")
+    dev = moves.device
+    if dev.type != "cuda" or moves.dtype != torch.int32 or moves.dim() != 2 or moves.shape[1] != 3 or not moves.is_contiguous():
+        raise ValueError(f"moves: a contiguous int32 [n, 3] tensor on a GPU is wanted, got {moves.dtype} {tuple(moves.shape)} on {dev}")
+    if (table is None) != (where is None):
+        raise ValueError("a table is rewritten by `where`: both or neither")
+    if table is not None and (table.dtype != torch.int32 or where.dtype != torch.int32 or table.device != dev or where.device != dev or not table.is_contiguous() or
+                              where.shape != (n_pages,) or not where.is_contiguous()):
+        raise ValueError(f"table: contiguous int32, where: int32 [{n_pages}], both on {dev}")
+    _lib.seq_call_on(dev, "umb_pages_copy", pools, pools.shape[0], moves, moves.shape[0], n_pages, table, 0 if table is None else table.numel(), where)
+
+
 class PagedSeqCache:
     """Paged key/value store, pooled blocks and recurrent-state slots for MANY sequences (the sequence-mixer models of
     libumbrella_seq.so; device-side statement: csrc/seq_common.h ``pkv_tok`` / ``pkv_blk``).
