@@ -227,12 +227,12 @@ def test_refusals_on_the_device():
 
 
 @pytest.mark.parametrize("kw", [dict(T=0), dict(N=0), dict(K=0), dict(S=0), dict(R=0), dict(R=129), dict(out=None), dict(base=None), dict(x=None), dict(a=None), dict(b=None),
-                                dict(adapter=None), dict(scratch=None), dict(floats=-1), dict(dtype=3)])
+                                dict(adapter=None), dict(scratch=None), dict(scratch=AT + 4), dict(floats=-1), dict(dtype=3)])
 def test_refusals_of_the_entry_point(kw):
     a = dict(T=4, N=8, K=16, S=2, R=8, out=AT, base=AT, x=AT, a=AT, b=AT, adapter=AT, scratch=AT, floats=0, dtype=1)
     a.update(kw)
     lib = _lib.load_seq()
-    n = lib.umb_seq_adapters_parts(4, 16) * 4 * 8 + a["floats"]
-    assert lib.umb_seq_adapters_parts(0, 8) == 0 and lib.umb_seq_adapters_parts(8, 0) == 0
+    n = lib.umb_seq_adapters_floats(4, 16, 8) + a["floats"]
+    assert lib.umb_seq_adapters_floats(0, 8, 8) == 0 and lib.umb_seq_adapters_floats(8, 0, 8) == 0 and lib.umb_seq_adapters_floats(8, 8, 129) == 0
     assert lib.umb_seq_adapters(a["out"], a["base"], a["x"], a["a"], a["b"], a["adapter"], None, None, a["T"], a["N"], a["K"], a["S"], a["R"], a["scratch"], n, a["dtype"],
                                 None) == EINVAL

@@ -394,11 +394,11 @@ SEQ_SIGNATURES = {
     "umb_sample_requests_bytes": [_I, _I],
     "umb_sample_requests": [_P, _P, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _L],
     "umb_pages_copy": [_P, _I, _P, _I, _I, _P, _L, _P],
-    "umb_seq_adapters_parts": [_I, _I],
+    "umb_seq_adapters_floats": [_I, _I, _I],
     "umb_seq_adapters": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _L, _I],
     "umb_seq_version": [],
 }
-_SEQ_NO_STREAM = {"umb_sample_requests_bytes", "umb_seq_adapters_parts", "umb_lat_attend_tiled_ok", "umb_seq_front_ok", "umb_seq_linear_split", "umb_seq_tile_kind", "umb_seq_tile_mix", "umb_lin_scan_columns", "umb_seq_resid_canon_step_ok", "umb_bsa_attend_tiled_ok", "umb_mingru_scratch_floats",
+_SEQ_NO_STREAM = {"umb_sample_requests_bytes", "umb_seq_adapters_floats", "umb_lat_attend_tiled_ok", "umb_seq_front_ok", "umb_seq_linear_split", "umb_seq_tile_kind", "umb_seq_tile_mix", "umb_lin_scan_columns", "umb_seq_resid_canon_step_ok", "umb_bsa_attend_tiled_ok", "umb_mingru_scratch_floats",
                   "umb_ssd_scan_chunked_floats", "umb_delta_scan_floats", "umb_gla_scan_chunked_floats"}          # predicates: no stream argument, the value is the answer
 _seq_lib = None
 

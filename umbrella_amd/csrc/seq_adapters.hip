@@ -3,16 +3,19 @@
 // x [T][K], A [S][R][K], B [S][N][R] in `dtype`; base and out fp32 [T][N]; of adapter a the first rank[a] of R count.  A row whose number is none of
 // 0 .. S - 1 is its base.
 //
-// Two launches: u = A x, fp32, summed over K in `parts` pieces; then out.  Rows of one adapter are taken together, up to 64, so that A and B are read once
-// for them: in a window of 256 rows the row whose place among its adapter's rows is a multiple of 64 stands for the 64 from it on, and every other row's
-// turn is empty.  Nothing has to be sorted or counted beforehand, and the order of a row's sums does not depend on which rows come with it.
+// Two launches: u = A x, fp32, summed over K in `parts` pieces; then out.  Rows of one adapter are taken together, so that A and B are read once for them.
+// Up to 256 rows: tiles of 16; the row whose place among its adapter's rows is a multiple of 16 stands for those from it on, and every other row's block is
+// empty: nothing is sorted or counted beforehand.  More rows: tiles of 64, and a launch in front works them out once for each window of 256.
+//
+// Bound by memory: x, A, B and the base are read once and out is written once, in pieces of 256 contiguous bytes and more, which fragments read from
+// memory directly (16 rows x 64 bytes) are not: they took 46 + 71 us where staging takes 10 + 16 (1999 tokens, fp16, 4096 x 4096, rank 32; 8192 tokens, bf16, 4096 x 6144, rank 64: 83 + 222, 30 + 107).
 //
 // u enters the second product with 22 bits or more: three bf16 terms (each the rest that the one before left), two fp16 ones behind a power of two per row
 // (whatever u's size), or itself in fp32.
 #include "seq_common.h"
 #include <algorithm>
 
-constexpr int WINDOW = 256, TILE = 64, R_MAX = 128;
+constexpr int WINDOW = 256, R_MAX = 128;
 
 template <typename P> struct Frag { u32x4 v; };
 template <> struct Frag<F32> { f32x4 lo, hi; };
@@ -24,28 +27,29 @@ template <> __device__ __forceinline__ f32x4 mma<F32>(const Frag<F32>& a, const 
   for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi[i], b.hi[i], c, 0, 0, 0);
   return c;
 }
-// eight elements p[0 .. n), nothing behind them
-template <typename P, bool WHOLE> __device__ __forceinline__ Frag<P> load8(const typename El<P>::type* p, int n) {
+// COUNT elements p[0 .. n), zeros behind them (WHOLE: all of them or none, 16-byte aligned)
+template <typename P, bool WHOLE, typename F, int COUNT> __device__ __forceinline__ F load_some(const typename El<P>::type* p, int n) {
+  typedef typename El<P>::type E;
+  static_assert(sizeof(F) == COUNT * sizeof(E));
+  u32x4 w[sizeof(F) / 16];
   if constexpr (WHOLE) {
-    Frag<P> f{};
-    if (n > 0) {
-      if constexpr (std::is_same_v<P, F32>) { f.lo = *reinterpret_cast<const f32x4*>(p); f.hi = *reinterpret_cast<const f32x4*>(p + 4); }
-      else f.v = *reinterpret_cast<const u32x4*>(p);
-    }
-    return f;
-  } else {
-    typename El<P>::type e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : (typename El<P>::type)0;
-    return __builtin_bit_cast(Frag<P>, e);
+    for (int i = 0; i < (int)(sizeof(F) / 16); ++i) w[i] = n > 0 ? reinterpret_cast<const u32x4*>(p)[i] : u32x4{0u, 0u, 0u, 0u};
+    return __builtin_bit_cast(F, w);
+  } else {
+    E e[COUNT];
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) e[i] = i < n ? p[i] : (E)0;
+    return __builtin_bit_cast(F, e);
   }
 }
 
-// The rows that block `i` of a window stands for: those of its own row's adapter from that row on, TILE at most, if the row's place among them is a multiple of
-// TILE; none otherwise.  rows: LDS [TILE]; all threads of 256 call it.
+// Rows of one adapter, TILE at most, in LDS `rows` [TILE]; n 0: none.  All threads of 256 call what makes one.
 struct Tile { int adapter, n; };
-__device__ __forceinline__ Tile rows_of(int t, int T, int S, const int* __restrict__ adapter, int* rows, int* waves) {
-  const int w0 = t / WINDOW * WINDOW, i = w0 + threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+
+// up to WINDOW rows: block t stands for the rows of row t's adapter from t on, if t's place among them is a multiple of TILE
+template <int TILE> __device__ __forceinline__ Tile tile_of_row(int t, int T, int S, const int* __restrict__ adapter, int* rows, int* waves) {
+  const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
   int mine = adapter[t], other = i < T ? adapter[i] : mine;
   if (mine < 0 || mine >= S) mine = -1;
   if (other < 0 || other >= S) other = -1;
@@ -65,209 +69,392 @@ __device__ __forceinline__ Tile rows_of(int t, int T, int S, const int* __restri
   return Tile{mine, min(TILE, all - first)};
 }
 
-// ---- u[part][t][r] = sum over the part's K of A x.  grid (rows, parts); a wave a quarter of the part's K where there are at most 16 rows, otherwise a quarter of
-// the rows
-template <typename P, bool WHOLE, int RF>
-__global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u, const typename El<P>::type* __restrict__ x, const typename El<P>::type* __restrict__ a,
-                                                           const int* __restrict__ adapter, const int* __restrict__ rank, int T, int K, int S, int R, int per) {
-  __shared__ int rows[TILE], waves[5];
-  __shared__ f32x4 part[3][RF][64];
-  const Tile tile = rows_of(blockIdx.x, T, S, adapter, rows, waves);
-  if (tile.n < 1 || tile.adapter < 0) return;
-  const int ra = rank ? min(max(rank[tile.adapter], 0), R) : R;
-  if (ra < 1) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const bool few = tile.n <= 16;
-  const int k0 = blockIdx.y * per, k1 = min(K, k0 + per);
-  // (steps of 32)
-  const int steps = (k1 - k0 + 31) / 32, s0 = few ? steps * wave / 4 : 0, s1 = few ? steps * (wave + 1) / 4 : steps;
-  const int own = few ? j : wave * 16 + j;
-  if (!few && wave * 16 >= tile.n) return;
-  const typename El<P>::type* xr = x + (long)rows[min(own, tile.n - 1)] * K;
-  const typename El<P>::type* ar[RF];
+// More rows: plan, of each window: how many tiles; their adapters; their first places and sizes (first + 1024 n); the window's rows, those of a tile side by
+// side.  A quarter of the window's rows is compared with each row by one of four threads.
+constexpr int PLAN_TILE = 64, PLAN_INTS = 1 + 3 * WINDOW;
+__global__ __launch_bounds__(4 * WINDOW) void adapter_plan_kernel(int* __restrict__ plan, const int* __restrict__ adapter, int T, int S) {
+  __shared__ __attribute__((aligned(16))) int ids[WINDOW], firsts[WINDOW];
+  __shared__ int said[4][3][WINDOW], waves[4];
+  const int i = threadIdx.x % WINDOW, q = threadIdx.x / WINDOW, t = blockIdx.x * WINDOW + i, lane = i & 63, wave = i >> 6;
+  int* p = plan + (long)blockIdx.x * PLAN_INTS;
+  int id = t < T ? adapter[t] : -2;
+  if (t < T && (id < 0 || id >= S)) id = -1;
+  if (q == 0) ids[i] = id;
+  __syncthreads();
+  int at = 0, n = 0, first = WINDOW;         // the row's place among its adapter's, how many those are, the first of them
+#pragma unroll 4
+  for (int j0 = (q + 1) * (WINDOW / 4) - 4; j0 >= q * (WINDOW / 4); j0 -= 4) {
+    const int4 v = *reinterpret_cast<const int4*>(ids + j0);
+    const int o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int f = 0; f < RF; ++f) ar[f] = a + ((long)tile.adapter * R + min(16 * f + j, ra - 1)) * K;
-  f32x4 acc[RF];
-#pragma unroll
-  for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = s0; s < s1; ++s) {
-    const int k = k0 + 32 * s + 8 * g, n = k1 - k;
-    const Frag<P> b = load8<P, WHOLE>(xr + k, n);
-#pragma unroll
-    for (int f = 0; f < RF; ++f)
-      if (16 * f < ra) acc[f] = mma<P>(load8<P, WHOLE>(ar[f] + k, n), b, acc[f]);
+    for (int e = 3; e >= 0; --e) {
+      const bool same = o[e] == id;
+      n += same;
+      at += same && j0 + e < i;
+      first = same ? j0 + e : first;
+    }
   }
-  if (few) {
-    if (wave > 0)
+  said[q][0][i] = at;
+  said[q][1][i] = n;
+  said[q][2][i] = first;
+  __syncthreads();
+  at = n = 0;
+  first = WINDOW;
 #pragma unroll
-      for (int f = 0; f < RF; ++f) part[wave - 1][f][lane] = acc[f];
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int f = 0; f < RF; ++f) acc[f] = (acc[f] + part[0][f][lane]) + (part[1][f][lane] + part[2][f][lane]);
+  for (int k = 0; k < 4; ++k) { at += said[k][0][i]; n += said[k][1][i]; first = min(first, said[k][2][i]); }
+  if (q == 0) firsts[i] = first;
+  __syncthreads();
+  // rows of an adapter stand together, adapters in the order of their first rows: in front of this row's are those whose first row is an earlier one
+  int front = 0;
+#pragma unroll 4
+  for (int j0 = q * (WINDOW / 4); j0 < (q + 1) * (WINDOW / 4); j0 += 4) {
+    const int4 v = *reinterpret_cast<const int4*>(firsts + j0);
+    front += (v.x < first) + (v.y < first) + (v.z < first) + (v.w < first);
   }
-  if (own >= tile.n) return;
-  float* to = u + ((long)blockIdx.y * T + rows[own]) * R;
+  said[q][0][i] = front;                     // (at is read by now: firsts stands between)
+  const bool leads = id != -2 && at % PLAN_TILE == 0;
+  const unsigned long long bal = __ballot(leads);
+  if (q == 0 && lane == 0) waves[wave] = __popcll(bal);
+  __syncthreads();
+  if (q > 0) return;
+  front = said[0][0][i] + said[1][0][i] + said[2][0][i] + said[3][0][i];
+  int k = __popcll(bal & ((1ull << lane) - 1ull)), all = 0;
 #pragma unroll
-  for (int f = 0; f < RF; ++f)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (16 * f + 4 * g + e < ra) to[16 * f + 4 * g + e] = acc[f][e];
+  for (int w = 0; w < 4; ++w) { if (w < wave) k += waves[w]; all += waves[w]; }
+  if (i == 0) p[0] = all;
+  if (leads) {
+    p[1 + k] = id;
+    p[1 + WINDOW + k] = front + at + 1024 * min(PLAN_TILE, n - at);
+  }
+  if (id != -2) p[1 + 2 * WINDOW + front + at] = t;
+}
+__device__ __forceinline__ Tile tile_of_plan(const int* __restrict__ p, int k, int* rows) {
+  const int said = p[1 + WINDOW + k], n = said / 1024, first = said % 1024;
+  __syncthreads();                           // (the tile before this one may still be read)
+  if ((int)threadIdx.x < n) rows[threadIdx.x] = p[1 + 2 * WINDOW + first + threadIdx.x];
+  __syncthreads();
+  return Tile{p[1 + k], n};
 }
 
-// ---- out = base + B (scale u).  grid (rows, pieces of N); a wave takes 16 columns at a time, all the tile's rows for them
+// each tile that is this block's: block = row, or, with a plan (TF 4), every slots-th tile of a window
+template <int TF, typename F>
+__device__ __forceinline__ void each_tile(const int* plan, int slots, int T, int S, const int* adapter, int* rows, int* waves, F f) {
+  if constexpr (TF == 1) {
+    const Tile t = tile_of_row<16>(blockIdx.y, T, S, adapter, rows, waves);
+    if (t.n > 0) f(t);
+  } else {
+    const int* p = plan + (long)(blockIdx.y / slots) * PLAN_INTS;
+    const int n = p[0];
+    for (int k = blockIdx.y % slots; k < n; k += slots) f(tile_of_plan(p, k, rows));
+  }
+}
+
+// ---- u[part][t][r] = sum over the part's K of A x.  grid (parts, rows or slots: the parts fastest, since blocks go round the eight dies and of a window's slots the first few alone have tiles).  Stages of KB bytes of K, of 16 TF tokens and 16 RF ranks, go through
+// registers to LDS, the next stage's loads in flight behind this one's products.  TF 4: a wave 16 of the tokens; 1: a quarter of the stage's K.
+template <typename P, bool WHOLE, int RF, int TF, int KB>
+__global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u, const typename El<P>::type* __restrict__ x, const typename El<P>::type* __restrict__ a,
+                                                           const int* __restrict__ adapter, const int* __restrict__ rank, const int* __restrict__ plan, int slots,
+                                                           int T, int K, int S, int R, int per) {
+  typedef typename El<P>::type E;
+  constexpr int ES = sizeof(E), KC = KB / ES, VE = 16 / ES, LD = KB + 16, STEPS = KC / 32, PER_ROW = KB / 16, ROWS = 256 / PER_ROW;
+  constexpr int NX = 16 * TF / ROWS > 0 ? 16 * TF / ROWS : 1, NA = 16 * RF / ROWS > 0 ? 16 * RF / ROWS : 1;
+  static_assert(16 % ROWS == 0 && (TF == 4 || STEPS % 4 == 0));
+  __shared__ int rows[16 * TF], waves[5];
+  __shared__ __attribute__((aligned(16))) char stage[(16 * TF + 16 * RF) * LD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  const int row = threadIdx.x / PER_ROW, piece = threadIdx.x % PER_ROW;
+  const int k0 = blockIdx.x * per, k1 = min(K, k0 + per);
+  each_tile<TF>(plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
+    if (tile.adapter < 0) return;
+    const int ra = rank ? min(max(rank[tile.adapter], 0), R) : R;
+    if (ra < 1) return;
+    const E* ap = a + (long)tile.adapter * R * K;
+    u32x4 xv[NX], av[NA];
+    // rows that are not there are zeros
+    auto load = [&](int k) __attribute__((always_inline)) {
+      const int at = k + piece * VE, left = k1 - at;
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int r = row + i * ROWS;
+        const bool in = r < tile.n;
+        xv[i] = load_some<P, WHOLE, u32x4, VE>(x + (long)rows[in ? r : 0] * K + at, in ? left : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        const int r = row + i * ROWS;
+        av[i] = load_some<P, WHOLE, u32x4, VE>(ap + (long)(r < ra ? r : 0) * K + at, r < ra ? left : 0);
+      }
+    };
+    f32x4 acc[RF];
+#pragma unroll
+    for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    load(k0);
+    for (int k = k0; k < k1; k += KC) {
+      if (k > k0) __syncthreads();           // (the stage before this one has been read)
+#pragma unroll
+      for (int i = 0; i < NX; ++i) *reinterpret_cast<u32x4*>(stage + (row + i * ROWS) * LD + piece * 16) = xv[i];
+#pragma unroll
+      for (int i = 0; i < NA; ++i) *reinterpret_cast<u32x4*>(stage + (16 * TF + row + i * ROWS) * LD + piece * 16) = av[i];
+      __syncthreads();
+      if (k + KC < k1) load(k + KC);
+      if (TF == 4 && wave * 16 >= tile.n) continue;
+      constexpr int MINE = TF == 4 ? STEPS : STEPS / 4;
+#pragma unroll
+      for (int s0 = 0; s0 < MINE; ++s0) {
+        const int s = TF == 4 ? s0 : wave * MINE + s0;
+        const char* at = stage + j * LD + (32 * s + 8 * g) * ES;
+        const Frag<P> b = *reinterpret_cast<const Frag<P>*>(at + (TF == 4 ? wave * 16 * LD : 0));
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+          if (16 * f < ra) acc[f] = mma<P>(*reinterpret_cast<const Frag<P>*>(at + (16 * TF + 16 * f) * LD), b, acc[f]);
+      }
+    }
+    if constexpr (TF == 1) {
+      __syncthreads();
+      f32x4(*part)[RF][64] = reinterpret_cast<f32x4(*)[RF][64]>(stage);
+      static_assert(3 * RF * 64 * 16 <= (16 + 16 * RF) * LD);
+      if (wave > 0)
+#pragma unroll
+        for (int f = 0; f < RF; ++f) part[wave - 1][f][lane] = acc[f];
+      __syncthreads();
+      if (wave > 0) return;
+#pragma unroll
+      for (int f = 0; f < RF; ++f) acc[f] = (acc[f] + part[0][f][lane]) + (part[1][f][lane] + part[2][f][lane]);
+    }
+    const int own = TF == 4 ? wave * 16 + j : j;
+    if (own >= tile.n) return;
+    float* to = u + ((long)blockIdx.x * T + rows[own]) * R;
+#pragma unroll
+    for (int f = 0; f < RF; ++f) {
+      const int r = 16 * f + 4 * g;
+      if (r + 4 <= ra && R % 4 == 0) *reinterpret_cast<f32x4*>(to + r) = acc[f];
+      else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (r + e < ra) to[r + e] = acc[f][e];
+    }
+  });
+}
+
+// ---- out = base + B (scale u).  grid (pieces of N, rows or slots).  Stages of CS columns: a wave's share of them for all the tile's rows goes to LDS, from where whole rows
+// leave, joined by the base (asked for in front of everything else).
 template <typename P> struct Terms { static constexpr int N = 1; };
 template <> struct Terms<BF16> { static constexpr int N = 3; };
 template <> struct Terms<F16> { static constexpr int N = 2; };
 
-template <typename P, bool WHOLE, bool QUADS, int RC>
+template <typename P, bool WHOLE, bool QUADS, int RC, int TF>
 __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float* base, const float* __restrict__ u, const typename El<P>::type* __restrict__ b,
-                                                         const int* __restrict__ adapter, const float* __restrict__ scale, const int* __restrict__ rank, int T, int N,
-                                                         int S, int R, int parts, int columns) {
+                                                         const int* __restrict__ adapter, const float* __restrict__ scale, const int* __restrict__ rank,
+                                                         const int* __restrict__ plan, int slots, int T, int N, int S, int R, int parts, int columns) {
   typedef typename El<P>::type E;
-  constexpr int NT = Terms<P>::N;
-  __shared__ int rows[TILE], waves[5];
-  __shared__ __attribute__((aligned(16))) E terms[NT][RC][TILE / 16][64][8];
-  __shared__ float power[TILE];
-  const Tile tile = rows_of(blockIdx.x, T, S, adapter, rows, waves);
-  if (tile.n < 1) return;
+  constexpr int NT = Terms<P>::N, CS = TF == 1 ? 256 : RC == 4 ? 64 : 128, LD = CS + 4, HF = CS / 64, NB = 16 * TF * CS / 1024, PER_ROW = CS / 4, ROWS = 256 / PER_ROW;
+  __shared__ int rows[16 * TF], waves[5];
+  __shared__ __attribute__((aligned(16))) E terms[NT][RC][TF][64][8];
+  __shared__ __attribute__((aligned(16))) float sums[16 * TF][LD];
+  __shared__ float power[16 * TF];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.y * columns, n1 = min(N, n0 + columns);
-  const int ra = tile.adapter < 0 ? 0 : rank ? min(max(rank[tile.adapter], 0), R) : R;
-  if (ra < 1) {
-    if (out != base)
-      for (int i = wave; i < tile.n; i += 4)
-        for (int n = n0 + lane; n < n1; n += 64) out[(long)rows[i] * N + n] = base[(long)rows[i] * N + n];
-    return;
-  }
-  const float sc = scale ? scale[tile.adapter] : 1.f;
-  // a row's terms by four lanes: lane j, g of the fragments is row j, elements 32 c + 8 g ..
-  const int i = threadIdx.x >> 2, q = threadIdx.x & 3;
-  float v[RC][8], most = 0.f;
+  const int row = threadIdx.x / PER_ROW, quad = threadIdx.x % PER_ROW;
+  const int n0 = blockIdx.x * columns, n1 = min(N, n0 + columns);
+  each_tile<TF>(plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
+    const int ra = tile.adapter < 0 ? 0 : rank ? min(max(rank[tile.adapter], 0), R) : R;
+    if (ra < 1 && out == base) return;
+    f32x4 x[NB];
+    Frag<P> w[HF][RC];
+    auto ask = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-  for (int c = 0; c < RC; ++c)
+      for (int i = 0; i < NB; ++i) {
+        const int r = row + i * ROWS, col = n + 4 * quad;
+        const float* o = base + (long)rows[r < tile.n ? r : 0] * N + col;
+        x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (r < tile.n) {
+          if (QUADS) { if (col < n1) x[i] = *reinterpret_cast<const f32x4*>(o); }
+          else
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int r = 32 * c + 8 * q + e;
-      float s = 0.f;
-      if (i < tile.n && r < ra) {
-        for (int p = 0; p < parts; ++p) s += u[((long)p * T + rows[i]) * R + r];
-        s *= sc;
-      }
-      v[c][e] = s;
-      most = fmaxf(most, fabsf(s));
-    }
-  if constexpr (NT == 2) {                   // fp16: the row's largest between 1 and 2
-    most = fmaxf(most, __shfl_xor(most, 1, 64));
-    most = fmaxf(most, __shfl_xor(most, 2, 64));
-    const int e = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
-    if (q == 0) power[i] = ldexpf(1.f, max(e, -126));
-#pragma unroll
-    for (int c = 0; c < RC; ++c)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[c][k] = ldexpf(v[c][k], -max(e, -126));
-  }
-#pragma unroll
-  for (int c = 0; c < RC; ++c)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      E* to = &terms[0][c][i >> 4][q * 16 + (i & 15)][e];
-      constexpr long next = (long)RC * (TILE / 16) * 64 * 8;
-      if constexpr (NT == 1) *to = v[c][e];
-      else {
-        float x = v[c][e];
-        const E hi = P::from_f(x);
-        to[0] = hi;
-        float rest = x - P::to_f(hi);
-        if (!(fabsf(rest) < INFINITY)) rest = 0.f;
-        if constexpr (NT == 2) to[next] = P::from_f(rest * 2048.f);
-        else {
-          const E mid = P::from_f(rest);
-          to[next] = mid;
-          to[2 * next] = P::from_f(rest - P::to_f(mid));
+            for (int e = 0; e < 4; ++e) if (col + e < n1) x[i][e] = o[e];
         }
       }
-    }
-  __syncthreads();
-  const int frags = (tile.n + 15) >> 4;
-  for (int n = n0 + 16 * wave; n < n1; n += 64) {
-    Frag<P> w[RC];
-    const E* br = b + ((long)tile.adapter * N + min(n + j, N - 1)) * R;
+      if (ra < 1) return;
 #pragma unroll
-    for (int c = 0; c < RC; ++c) w[c] = load8<P, WHOLE>(br + 32 * c + 8 * g, (WHOLE ? (ra + 7) & ~7 : ra) - 32 * c - 8 * g);
-    if (WHOLE && (ra & 7)) {                 // what stands behind the rank is nobody's
+      for (int h = 0; h < HF; ++h) {
+        const E* br = b + ((long)tile.adapter * N + min(n + 16 * (wave * HF + h) + j, N - 1)) * R;
 #pragma unroll
-      for (int c = 0; c < RC; ++c) {
-        E e[8];
-        __builtin_memcpy(e, &w[c], sizeof e);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) if (32 * c + 8 * g + k >= ra) e[k] = (E)0;
-        __builtin_memcpy(&w[c], e, sizeof e);
+        for (int c = 0; c < RC; ++c) w[h][c] = load_some<P, WHOLE, Frag<P>, 8>(br + 32 * c + 8 * g, (WHOLE ? (ra + 7) & ~7 : ra) - 32 * c - 8 * g);
       }
-    }
+    };
+    ask(n0);
+    if (ra > 0) {
+      const float sc = scale ? scale[tile.adapter] : 1.f;
+      // a row's terms by four lanes (64 rows), or one of 16 rows by sixteen: lane j, g of the fragments is row j, elements 32 c + 8 g ..
+      const int i = threadIdx.x >> 2, q = threadIdx.x & 3;
+      if (i < 16 * TF) {
+        float v[RC][8], most = 0.f;
 #pragma unroll
-    for (int f = 0; f < TILE / 16; ++f) {
-      if (f >= frags) break;
-      const int at = f * 16 + j, col = n + 4 * g;
-      const bool in = at < tile.n;
-      const long o = (long)rows[in ? at : 0] * N + col;
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-      if (in) {
-        if (QUADS) { if (col < n1) x = *reinterpret_cast<const f32x4*>(base + o); }
+        for (int c = 0; c < RC; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+        if (i < tile.n) {
+          const float* ur = u + (long)rows[i] * R;
+#pragma unroll 4
+          for (int p = 0; p < parts; ++p, ur += (long)T * R)
+#pragma unroll
+            for (int c = 0; c < RC; ++c) {
+              const int r = 32 * c + 8 * q;
+              if (r + 8 <= ra && R % 4 == 0) {
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(ur + r), hi = *reinterpret_cast<const f32x4*>(ur + r + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[c][e] += lo[e]; v[c][4 + e] += hi[e]; }
+              } else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) if (r + e < ra) v[c][e] += ur[r + e];
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < RC; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[c][e] *= sc;
+            most = fmaxf(most, fabsf(v[c][e]));
+          }
+        if constexpr (NT == 2) {             // fp16: the row's largest between 1 and 2
+          most = fmaxf(most, __shfl_xor(most, 1, 64));
+          most = fmaxf(most, __shfl_xor(most, 2, 64));
+          const int e = most > 0.f && most < INFINITY ? max(ilogbf(most), -126) : 0;
+          if (q == 0) power[i] = ldexpf(1.f, e);
+#pragma unroll
+          for (int c = 0; c < RC; ++c)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[c][k] = ldexpf(v[c][k], -e);
+        }
+#pragma unroll
+        for (int c = 0; c < RC; ++c) {
+          E t[NT][8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if constexpr (NT == 1) t[0][e] = v[c][e];
+            else {
+              t[0][e] = P::from_f(v[c][e]);
+              float rest = v[c][e] - P::to_f(t[0][e]);
+              if (!(fabsf(rest) < INFINITY)) rest = 0.f;
+              if constexpr (NT == 2) t[1][e] = P::from_f(rest * 2048.f);
+              else {
+                t[1][e] = P::from_f(rest);
+                t[2][e] = P::from_f(rest - P::to_f(t[1][e]));
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < NT; ++k) __builtin_memcpy(&terms[k][c][i >> 4][q * 16 + (i & 15)][0], t[k], sizeof t[k]);
+        }
+      }
+      __syncthreads();
+    }
+    const int frags = TF == 1 ? 1 : (tile.n + 15) >> 4;
+    for (int n = n0; n < n1; n += CS) {
+      if (ra > 0) {
+        if (WHOLE && (ra & 7)) {             // what stands behind the rank is nobody's
+#pragma unroll
+          for (int h = 0; h < HF; ++h)
+#pragma unroll
+            for (int c = 0; c < RC; ++c) {
+              E e[8];
+              __builtin_memcpy(e, &w[h][c], sizeof e);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) if (32 * c + 8 * g + k >= ra) e[k] = (E)0;
+              __builtin_memcpy(&w[h][c], e, sizeof e);
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < TF; ++f) {
+          if (f >= frags) break;
+          f32x4 acc[HF], low[HF];
+#pragma unroll
+          for (int h = 0; h < HF; ++h) acc[h] = low[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < RC; ++c) {
+            const Frag<P>* t = reinterpret_cast<const Frag<P>*>(&terms[0][c][f][lane][0]);
+            constexpr long next = (long)RC * TF * 64;
+            const Frag<P> t0 = t[0];
+#pragma unroll
+            for (int h = 0; h < HF; ++h) acc[h] = mma<P>(w[h][c], t0, acc[h]);
+#pragma unroll
+            for (int k = NT - 1; k > 0; --k) {
+              const Frag<P> tk = t[k * next];
+#pragma unroll
+              for (int h = 0; h < HF; ++h) low[h] = mma<P>(w[h][c], tk, low[h]);
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < HF; ++h) {
+            if constexpr (NT == 3) acc[h] += low[h];
+            if constexpr (NT == 2) acc[h] = (acc[h] + low[h] * (1.f / 2048.f)) * power[f * 16 + j];
+            *reinterpret_cast<f32x4*>(&sums[f * 16 + j][16 * (wave * HF + h) + 4 * g]) = acc[h];
+          }
+        }
+        __syncthreads();
+      }
+      f32x4 y[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int r = row + i * ROWS;
+        y[i] = x[i];
+        if (ra > 0 && r < tile.n) y[i] += *reinterpret_cast<const f32x4*>(&sums[r][4 * quad]);
+      }
+      if (n + CS < n1) ask(n + CS);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int r = row + i * ROWS, col = n + 4 * quad;
+        if (r >= tile.n) continue;
+        float* o = out + (long)rows[r] * N + col;
+        if (QUADS) { if (col < n1) *reinterpret_cast<f32x4*>(o) = y[i]; }
         else
 #pragma unroll
-          for (int e = 0; e < 4; ++e) if (col + e < n1) x[e] = base[o + e];
+          for (int e = 0; e < 4; ++e) if (col + e < n1) o[e] = y[i][e];
       }
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f}, low = acc;
-#pragma unroll
-      for (int c = 0; c < RC; ++c) {
-        const Frag<P>* t = reinterpret_cast<const Frag<P>*>(&terms[0][c][f][lane][0]);
-        constexpr long next = (long)RC * (TILE / 16) * 64;
-        if constexpr (NT == 3) {
-          low = mma<P>(w[c], t[2 * next], low);
-          low = mma<P>(w[c], t[next], low);
-          acc = mma<P>(w[c], t[0], acc);
-        } else {
-          if constexpr (NT == 2) low = mma<P>(w[c], t[next], low);
-          acc = mma<P>(w[c], t[0], acc);
-        }
-      }
-      if constexpr (NT == 3) acc += low;
-      if constexpr (NT == 2) acc = (acc + low * (1.f / 2048.f)) * power[at];
-      if (!in) continue;
-      x += acc;
-      if (QUADS) { if (col < n1) *reinterpret_cast<f32x4*>(out + o) = x; }
-      else
-#pragma unroll
-        for (int e = 0; e < 4; ++e) if (col + e < n1) out[o + e] = x[e];
+      __syncthreads();                       // (the next stage's sums, the next tile's terms)
     }
-  }
+  });
 }
 
-extern "C" int umb_seq_adapters_parts(int T, int K) {
-  if (T < 1 || K < 1) return 0;
-  const int steps = (K + 31) / 32, want = std::max(1, 512 / std::min(T, 512));
-  return std::max(1, std::min({want, (steps + 3) / 4, 16}));
+static int adapter_parts(int T, int K) { return std::max(1, std::min(T > 4096 ? 4 : 8, (K + 511) / 512)); }
+static long plan_ints(int T) { return T > WINDOW ? (long)((T + WINDOW - 1) / WINDOW) * PLAN_INTS : 0; }
+
+extern "C" long umb_seq_adapters_floats(int T, int K, int R) {
+  return T < 1 || T > (1 << 20) || K < 1 || R < 1 || R > R_MAX ? 0 : (((long)adapter_parts(T, K) * T * R + 3) & ~3L) + plan_ints(T);
 }
 
-template <typename P, bool WHOLE>
+template <typename P, bool WHOLE, int TF>
 static int adapters_launch(float* out, const float* base, const void* x, const void* a, const void* b, const int* adapter, const float* scale, const int* rank, int T,
                            int N, int K, int S, int R, bool quads, float* u, hipStream_t st) {
   typedef typename El<P>::type E;
-  const int parts = umb_seq_adapters_parts(T, K), per = (((K + 31) / 32 + parts - 1) / parts) * 32;
-#define DOWN(RF) hipLaunchKernelGGL((adapter_down_kernel<P, WHOLE, RF>), dim3(T, parts), dim3(256), 0, st, u, (const E*)x, (const E*)a, adapter, rank, T, K, S, R, per)
-  if (R <= 16) DOWN(1);
-  else if (R <= 32) DOWN(2);
-  else if (R <= 64) DOWN(4);
-  else DOWN(8);
+  const int parts = adapter_parts(T, K), per = (((K + 31) / 32 + parts - 1) / parts) * 32;
+  int* plan = nullptr;
+  int slots = 1, blocks = T, tiles = T;
+  if (TF > 1) {
+    plan = reinterpret_cast<int*>(u + (((long)parts * T * R + 3) & ~3L));
+    const int windows = (T + WINDOW - 1) / WINDOW;
+    slots = T <= 2048 ? 32 : 8;
+    blocks = windows * slots;
+    tiles = (T + PLAN_TILE - 1) / PLAN_TILE;
+    hipLaunchKernelGGL(adapter_plan_kernel, dim3(windows), dim3(4 * WINDOW), 0, st, plan, adapter, T, S);
+    UMB_LAUNCH_CHECK();
+  }
+#define DOWN(RF, KB)                                                                                                                                       \
+  hipLaunchKernelGGL((adapter_down_kernel<P, WHOLE, RF, TF, KB>), dim3(parts, blocks), dim3(256), 0, st, u, (const E*)x, (const E*)a, adapter, rank, plan, slots, \
+                     T, K, S, R, per)
+  // bytes of K a stage: 8 to 12 loads a thread in flight, and for few tokens the least stages
+  if (R <= 16) DOWN(1, (TF == 1 ? 1024 : 512));
+  else if (R <= 32) DOWN(2, 512);
+  else if (R <= 64) DOWN(4, (TF == 1 ? 512 : 256));
+  else DOWN(8, (TF == 1 && !std::is_same_v<P, F32> ? 256 : TF == 1 ? 512 : 256));
 #undef DOWN
   UMB_LAUNCH_CHECK();
-  const int columns = 256 * (1 + (N - 1) / (256 * 65535)), pieces = (N + columns - 1) / columns;
-#define UP(RC)                                                                                                                                        \
-  if (quads) hipLaunchKernelGGL((adapter_up_kernel<P, WHOLE, true, RC>), dim3(T, pieces), dim3(256), 0, st, out, base, u, (const E*)b, adapter, scale, rank, \
-                                T, N, S, R, parts, columns);                                                                                          \
-  else hipLaunchKernelGGL((adapter_up_kernel<P, WHOLE, false, RC>), dim3(T, pieces), dim3(256), 0, st, out, base, u, (const E*)b, adapter, scale, rank, T, N, \
-                          S, R, parts, columns)
+  int columns = 256;
+  while (columns < 1024 && (long)tiles * (N / (2 * columns)) >= 1024) columns *= 2;
+  const int pieces = (N + columns - 1) / columns;
+#define UP(RC)                                                                                                                                             \
+  if (quads) hipLaunchKernelGGL((adapter_up_kernel<P, WHOLE, true, RC, TF>), dim3(pieces, blocks), dim3(256), 0, st, out, base, u, (const E*)b, adapter, scale, \
+                                rank, plan, slots, T, N, S, R, parts, columns);                                                                            \
+  else hipLaunchKernelGGL((adapter_up_kernel<P, WHOLE, false, RC, TF>), dim3(pieces, blocks), dim3(256), 0, st, out, base, u, (const E*)b, adapter, scale, rank, \
+                          plan, slots, T, N, S, R, parts, columns)
   if (R <= 32) { UP(1); }
   else if (R <= 64) { UP(2); }
   else { UP(4); }
@@ -278,13 +465,13 @@ static int adapters_launch(float* out, const float* base, const void* x, const v
 
 extern "C" int umb_seq_adapters(float* out, const float* base, const void* x, const void* a, const void* b, const int* adapter, const float* scale, const int* rank,
                                 int T, int N, int K, int S, int R, float* scratch, long scratch_floats, int dtype, hipStream_t st) {
-  if (!out || !base || !x || !a || !b || !adapter || !scratch || T < 1 || N < 1 || K < 1 || S < 1 || R < 1 || R > R_MAX || N > (1 << 24) || K > (1 << 24) ||
-      scratch_floats < (long)umb_seq_adapters_parts(T, K) * T * R)
+  if (!out || !base || !x || !a || !b || !adapter || !scratch || T < 1 || T > (1 << 20) || N < 1 || K < 1 || S < 1 || R < 1 || R > R_MAX || N > (1 << 24) || K > (1 << 24) ||
+      (uintptr_t)scratch % 16 || scratch_floats < umb_seq_adapters_floats(T, K, R))
     return UMB_EINVAL;
   const bool quads = N % 4 == 0 && ((uintptr_t)out | (uintptr_t)base) % 16 == 0;
   const bool whole = K % 8 == 0 && R % 8 == 0 && ((uintptr_t)x | (uintptr_t)a | (uintptr_t)b) % 16 == 0;
   DISPATCH_SEQ_DTYPE(dtype, {
-    return whole ? adapters_launch<P, true>(out, base, x, a, b, adapter, scale, rank, T, N, K, S, R, quads, scratch, st)
-                 : adapters_launch<P, false>(out, base, x, a, b, adapter, scale, rank, T, N, K, S, R, quads, scratch, st);
+    auto launch = T <= WINDOW ? (whole ? adapters_launch<P, true, 1> : adapters_launch<P, false, 1>) : (whole ? adapters_launch<P, true, 4> : adapters_launch<P, false, 4>);
+    return launch(out, base, x, a, b, adapter, scale, rank, T, N, K, S, R, quads, scratch, st);
   })
 }

@@ -57,7 +57,7 @@ def add_adapters(base, x, a, b, adapter, scale=None, rank=None, out=None):
         if t is not None and (t.device != dev or not t.is_contiguous()):
             raise ValueError("contiguous tensors on one device are wanted")
     if T:
-        n = _lib.load_seq().umb_seq_adapters_parts(T, K) * T * R
+        n = _lib.load_seq().umb_seq_adapters_floats(T, K, R)
         scratch = torch.empty(n, dtype=torch.float32, device=dev)
         _lib.seq_call_on(dev, "umb_seq_adapters", out, base, x, a, b, adapter, scale, rank, T, N, K, S, R, scratch, n, code)
     return out
