@@ -4,9 +4,20 @@
 // in front of which less than p of the first k's mass stands; those with w >= m.  The shortest prefix is kept, and of it the first token whose mass,
 // with all in front of it, exceeds u times the kept mass is drawn.
 //
-// Weights are 64-bit floats, summed as whole numbers of 2^-44 of the largest: such sums are the same in any order, and a border between two tokens
-// falls where a 64-bit sum of any order puts it but for some 1e-12 of the mass.  (In 32 bits a flat row of 128256 values has thousands of borders that
-// the sum's order moves.)
+// Weights are 64-bit floats, summed as whole numbers: such sums are the same in any order, and a border between two tokens falls where a 64-bit sum of
+// any order puts it but for some 1e-12 of the mass.  (In 32 bits a flat row of 128256 values has thousands of borders that the sum's order moves.)
+//
+// Nothing is sorted but what stands next to a border.  Three launches:
+//   slices   a row in slices, each read once into registers: its largest, and counts and masses of bins an eighth of T wide, 256 below the largest (what is
+//            further down weighs less than 2^-46 of the row).  Bins lie on one lattice, floor(8 x / T), and masses are relative to their bin's middle, so
+//            that slices' add up as whole numbers, count and mass in one 64-bit atomic
+//   collect  the row's bins, summed up from the top, say which bins hold the k-th value, the ends of top-p and min-p and the token drawn (intervals, since
+//            the mass behind p and u is known to a bin only); their tokens are collected, from slices that have any.  A row of a small k has counts alone, and
+//            all tokens down to the k-th value's bin are collected
+//   resolve  a row's collected tokens by one workgroup: where they are many, bins again, up to 256 in each bin; then in order: the exact ends, then the draw
+// Bound by the logits: the first launch reads them from memory, the second a part of them again, from the cache behind it.
+// Rows of up to SMALL_V values are taken whole by the last launch alone.  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
+// the thousand), is searched eight bits of the key at a time, by one workgroup.
 #include "seq_common.h"
 #include <algorithm>
 
@@ -114,38 +125,14 @@ __device__ Pick find_in_row(const float* __restrict__ row, int V, float top, dou
   return got;
 }
 
-// one workgroup a row
-__global__ __launch_bounds__(ST) void sample_requests_kernel(int* __restrict__ tokens, float* __restrict__ probs, const float* __restrict__ logits, long ld, int V,
-                                                             const float* __restrict__ uniforms, const float* __restrict__ temperature,
-                                                             const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p) {
-  __shared__ unsigned cnt[256];
-  __shared__ unsigned long long sum[256];
-  __shared__ __attribute__((aligned(16))) int shared[8];
-  __shared__ unsigned long long wide[16];
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float* row = logits + (long)r * ld;
-  const RowSettings s = row_settings(r, V, temperature, top_k, top_p, min_p, uniforms);
-  unsigned best = 0u;
-  int at = V;
-  for (int i = tid; i < V; i += ST) {
-    const unsigned k = key_of(row[i]);
-    if (k > best) { best = k; at = i; }
-  }
-  unsigned long long b = ((unsigned long long)best << 32) | (unsigned)(0x7fffffff - at);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { const unsigned long long x = __shfl_xor(b, o, 64); b = x > b ? x : b; }
-  if (lane == 0) wide[wave] = b;
-  __syncthreads();
-  for (int i = 0; i < 16; ++i) b = wide[i] > b ? wide[i] : b;
-  const unsigned top_key = (unsigned)(b >> 32);
-  const float top = of_key(top_key);
-  if (top_key <= KEY_NONE || s.greedy) {
-    if (tid == 0) {
-      tokens[r] = top_key <= KEY_NONE ? -1 : 0x7fffffff - (int)(b & 0xffffffffu);
-      if (probs) probs[r] = top_key <= KEY_NONE ? 0.f : 1.f;
-    }
-    return;
-  }
+// the whole of a row by one workgroup, some eleven passes over it
+struct SlowRoom { unsigned cnt[256]; unsigned long long sum[256]; unsigned long long wide[16]; int shared[8]; };
+__device__ __attribute__((noinline)) void sample_slow(int r, int* __restrict__ tokens, float* __restrict__ probs, const float* __restrict__ row, int V, RowSettings s,
+                                                      float top, SlowRoom& room) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  unsigned* cnt = room.cnt;
+  unsigned long long *sum = room.sum, *wide = room.wide;
+  int* shared = room.shared;
   // everything's and min-p's counts and masses
   __syncthreads();
   if (tid < 4) wide[tid] = 0ull;
@@ -198,7 +185,736 @@ __global__ __launch_bounds__(ST) void sample_requests_kernel(int* __restrict__ t
   }
 }
 
-extern "C" long umb_sample_requests_bytes(int rows, int V) { return rows < 1 || V < 1 || V > SAMPLE_VMAX ? 0 : 16; }
+// ------------------------------------------------------------------ bins
+constexpr int BINS = 256, SMALL_V = 2048, CAP = 2048, K_COUNT = 1024, P_MAX = 64;
+constexpr double PER_T = 8.0, LATTICE = 1099511627776.0;         // bins a T; beyond 2^40 neighbouring floats are 2^16 bins apart and more
+constexpr double MAGIC = 4503599627370496.0;                     // 2^52: added to a number below 2^51, it leaves the nearest whole number in the low bits
+constexpr double BIN_ONE = 4294967296.0;                         // a bin's masses, in 2^-32 of its middle's weight: 48 bits for 2^15 of them, 16 above for their number
+constexpr double FINE_ONE = 70368744177664.0;                    // 2^46, of the row's largest weight
+
+// e^(f / 8) of -0.5 <= f <= 0.5: Taylor's sum to the sixth power, good to 1e-12 of it
+__device__ __forceinline__ double exp_bin(double f) {
+  constexpr double c = 1.0 / PER_T;
+  double p = c * c * c * c * c * c / 720.0;
+  p = fma(p, f, c * c * c * c * c / 120.0);
+  p = fma(p, f, c * c * c * c / 24.0);
+  p = fma(p, f, c * c * c / 6.0);
+  p = fma(p, f, c * c / 2.0);
+  p = fma(p, f, c);
+  return fma(p, f, 1.0);
+}
+// e^d of -40 < d <= 0.1 to some 2e-15 of it (a power of two times Taylor's sum to the 12th power of a rest of at most 0.347), 0 below
+__device__ __forceinline__ double exp_down(double d) {
+  if (!(d > -40.0)) return 0.0;
+  const double n = rint(d * 1.4426950408889634074);
+  const double r = fma(-n, 2.3190468138462996e-17, fma(-n, 0.69314718055994530942, d));
+  double p = 1.0 / 479001600.0;
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return p * __longlong_as_double((long long)(1023 + (int)n) << 52);
+}
+// a value's weight beside the row's largest; values of an infinite one's row weigh nothing but for the infinite ones
+__device__ __forceinline__ double weight_at(float x, float top, double inv_t) {
+  return x == top ? 1.0 : top < INFINITY ? exp_down(((double)x - (double)top) * inv_t) : 0.0;
+}
+__device__ __forceinline__ unsigned long long fine_of(double w) {
+  return (unsigned long long)__double_as_longlong(fma(w, FINE_ONE, MAGIC)) & 0xfffffffffffffull;
+}
+// whether a value weighs anything beside `top`, as far as infinities and the lattice's end tell
+__device__ __forceinline__ bool counts(float x, float top, double per) {
+  return x > -INFINITY && (x == top || (top < INFINITY && fabs((double)x * per) < LATTICE));
+}
+// where a value lies on the lattice; monotone in x, whatever T is
+__device__ __forceinline__ double line_of(float x, double per) { return x < INFINITY ? fmin(fmax((double)x * per, -LATTICE), LATTICE) : LATTICE; }
+
+// the least float x of which x per >= goal, a whole number
+__device__ __forceinline__ float least_at(double goal, double per) {
+  const double v = goal / per;
+  if (v >= 3.4028235e38) return INFINITY;
+  unsigned k = key_of(v > -3.4028235e38 ? (float)v : -3.402823466e38f);
+  for (int i = 0; i < 4 && (double)of_key(k) * per < goal; ++i) ++k;
+  for (int i = 0; i < 4 && k > KEY_NONE + 1 && (double)of_key(k - 1) * per >= goal; ++i) --k;
+  return of_key(k);
+}
+
+struct SliceHead { float top; int at, found, pad; };
+// what collect leaves for resolve; `mass` and `count`: in front of each bin
+struct RowSaid {
+  double all;
+  int count_all, slots, k_binds, k0, m0, m1; // k_binds 2: the k-th is the last of bin k0
+  int p_binds, m_binds, whole, pad;          // whole: everything down to the last collected token is collected
+};
+struct RowSums {
+  double mass[BINS];
+  int count[BINS];
+  short slot[BINS];                          // its place among the bins that are collected, -1: it is not
+  RowSaid said;
+};
+static_assert(sizeof(RowSums) % 16 == 0 && sizeof(RowSaid) % 16 == 0);
+struct Scratch { SliceHead* heads; unsigned long long *bins, *found; RowSums* sums; };
+__host__ __device__ __forceinline__ long row_bytes(int P, int slice) { return (long)P * (16 + BINS * 8 + slice / 4 * 8) + (long)sizeof(RowSums); }
+__device__ __forceinline__ Scratch scratch_of(char* base, int row, int P, int slice) {
+  char* p = base + row * row_bytes(P, slice);
+  Scratch s;
+  s.bins = reinterpret_cast<unsigned long long*>(p);
+  s.found = s.bins + (long)P * BINS;
+  s.sums = reinterpret_cast<RowSums*>(s.found + (long)P * (slice / 4));
+  s.heads = reinterpret_cast<SliceHead*>(s.sums + 1);
+  return s;
+}
+
+// a slice's values in registers: element e of thread t is value index_of(e); -inf behind the row's end and for NaN
+template <int NT, int NE, bool VEC> __device__ __forceinline__ int index_of(int base, int e) {
+  return VEC ? base + ((e >> 2) * NT + (int)threadIdx.x) * 4 + (e & 3) : base + e * NT + (int)threadIdx.x;
+}
+template <int NT, int NE, bool VEC> __device__ __forceinline__ void load_slice(float (&x)[NE], const float* __restrict__ row, int base, int V) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int e = 0; e < NE; e += 4) {
+      const int i = index_of<NT, NE, VEC>(base, e);
+      f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (i + 3 < V) v = *reinterpret_cast<const f32x4*>(row + i);
+      else
+#pragma unroll
+        for (int k = 0; k < 3; ++k) if (i + k < V) v[k] = row[i + k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[e + k] = v[k];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const int i = index_of<NT, NE, VEC>(base, e);
+      x[e] = i < V ? row[i] : -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < NE; ++e) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
+}
+
+// grid (slices, rows)
+template <int NT, int NE, bool VEC>
+__global__ __launch_bounds__(NT) void sample_slices_kernel(char* __restrict__ scratch, const float* __restrict__ logits, long ld, int V,
+                                                           const float* __restrict__ temperature, const int* __restrict__ top_k) {
+  constexpr int COPIES = 4;                  // of each bin, by lane: a row's values crowd in a few dozen bins
+  __shared__ unsigned long long bins[COPIES * BINS];
+  __shared__ float tops[NT / 64];
+  __shared__ int at;
+  const int r = blockIdx.y, P = gridDim.x, p = blockIdx.x, base = p * NT * NE, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float x[NE];
+  load_slice<NT, NE, VEC>(x, logits + (long)r * ld, base, V);
+  for (int i = threadIdx.x; i < COPIES * BINS; i += NT) bins[i] = 0ull;
+  if (threadIdx.x == 0) at = 0x7fffffff;
+  float top = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < NE; ++e) top = fmaxf(top, x[e]);
+  top = wave_max(top);
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) top = fmaxf(top, tops[w]);
+  const Scratch s = scratch_of(scratch, r, P, NT * NE);
+  const float t = temperature ? temperature[r] : 1.f;
+  if (!(t > 0.f)) {                          // the first of the largest
+#pragma unroll
+    for (int e = 0; e < NE; ++e) if (x[e] == top) atomicMin(&at, index_of<NT, NE, VEC>(base, e));
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) s.heads[p] = SliceHead{top, at, 0, 0};
+  if (!(top > -INFINITY) || !(t > 0.f)) return;
+  const double per = PER_T / (double)t, first = floor(line_of(top, per));
+  const int k = top_k ? top_k[r] : 0;
+  unsigned long long* const mine = bins + (threadIdx.x & (COPIES - 1));
+  auto count = [&](int j, unsigned long long v) __attribute__((always_inline)) { atomicAdd(mine + COPIES * j, v); };
+  if (top == INFINITY || !(fabs((double)top * per) < LATTICE)) {   // its equals alone count
+#pragma unroll
+    for (int e = 0; e < NE; ++e) if (x[e] == top) count(0, 1ull << 48);
+  } else if (k >= 1 && k <= K_COUNT) {
+    // (-inf, and what the lattice does not reach, are far below)
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const double j = first - floor((double)x[e] * per);
+      if (j < BINS) atomicAdd(reinterpret_cast<unsigned*>(mine + COPIES * (int)j) + 1, 1u << 16);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const double l = (double)x[e] * per, f = floor(l), j = first - f;
+      if (j < BINS) count((int)j, (1ull << 48) + ((unsigned long long)__double_as_longlong(fma(exp_bin(l - f - 0.5), BIN_ONE, MAGIC)) & 0x7ffffffffffffull));
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < BINS) {
+    unsigned long long sum = 0ull;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) sum += bins[COPIES * threadIdx.x + i];
+    s.bins[p * BINS + threadIdx.x] = sum;
+  }
+}
+
+// how many of `n` bins in a row, NB a thread, have what holds for the first of them and not for the rest
+template <int NB> __device__ __forceinline__ int bins_with(const bool (&holds)[NB]) {
+  int n = 0;
+#pragma unroll
+  for (int e = 0; e < NB; ++e) n += __syncthreads_count(holds[e]);
+  return n;
+}
+
+// grid (slices, rows)
+template <int NT, int NE, bool VEC>
+__global__ __launch_bounds__(NT) void sample_collect_kernel(char* __restrict__ scratch, const float* __restrict__ logits, long ld, int V, const float* __restrict__ uniforms,
+                                                            const float* __restrict__ temperature, const int* __restrict__ top_k, const float* __restrict__ top_p,
+                                                            const float* __restrict__ min_p) {
+  constexpr int SLICE_CAP = NT * NE / 4;
+  __shared__ double m_in[BINS], wave_m[4];
+  __shared__ int shift[P_MAX], c_in[BINS], wave_c[4], wave_s[4], found;
+  __shared__ float bounds[4][2];
+  const int r = blockIdx.y, P = gridDim.x, p = blockIdx.x, b = threadIdx.x, lane = b & 63, wave = b >> 6;
+  const RowSettings set = row_settings(r, V, temperature, top_k, top_p, min_p, uniforms);
+  if (set.greedy) return;
+  const Scratch s = scratch_of(scratch, r, P, NT * NE);
+  // few rows wait for their loads one after the other: the slice is asked for early, wanted or not
+  constexpr bool EARLY = NE <= 16;
+  float x[NE];
+  const int base = p * NT * NE;
+  if constexpr (EARLY) load_slice<NT, NE, VEC>(x, logits + (long)r * ld, base, V);
+  const float head = lane < P ? s.heads[lane].top : -INFINITY, top = wave_max(head);
+  if (!(top > -INFINITY)) return;
+  const bool bin = b < BINS;
+  const double per = PER_T / set.t, line = line_of(top, per), first = floor(line);
+  if (b < P) {
+    const double d = first - floor(line_of(head, per));
+    shift[b] = d < BINS && counts(head, top, per) ? (int)d : BINS;
+  }
+  if (b == 0) found = 0;
+  __syncthreads();
+  int c = 0;
+  unsigned long long q = 0ull;
+  if (bin) {
+#pragma unroll 8
+    for (int i = 0; i < P; ++i) {
+      const int k = b - shift[i];
+      const unsigned long long v = s.bins[i * BINS + max(k, 0)];
+      if (k >= 0) {
+        c += (int)(v >> 48);
+        q += v & 0xffffffffffffull;
+      }
+    }
+  }
+  // a bin's middle beside the largest; beside an infinite one, or one beyond the lattice, only its equals count
+  const bool flat = top == INFINITY || !(fabs((double)top * per) < LATTICE);
+  double m = !bin ? 0.0 : flat ? (b == 0 ? (double)c : 0.0) : (double)q * (1.0 / BIN_ONE) * exp_down((first - b + 0.5 - line) * (1.0 / PER_T));
+  const int c_own = c;
+  if (bin) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int cc = __shfl_up(c, o, 64);
+      const double mm = __shfl_up(m, o, 64);
+      if (lane >= o) { c += cc; m += mm; }
+    }
+    if (lane == 63) { wave_c[wave] = c; wave_m[wave] = m; }
+  }
+  __syncthreads();
+  if (bin) {
+    for (int w = 0; w < wave; ++w) { c += wave_c[w]; m += wave_m[w]; }
+    c_in[b] = c;
+    m_in[b] = m;
+  }
+  __syncthreads();
+  const int c_all = c_in[BINS - 1];
+  const double all = m_in[BINS - 1], slack = 1e-11 * all, m_ex = b > 0 && bin ? m_in[b - 1] : 0.0;
+  // the bins that each end may lie in: k0, [p0, p1], [m0, m1], [d0, d1]; BINS: nowhere
+  const int k = set.m > 1.0 ? 1 : set.k;
+  const bool whole = top_k && top_k[r] >= 1 && top_k[r] <= K_COUNT, k_binds = k < c_all;
+  const int k0 = k_binds ? __syncthreads_count(bin && c < k) : BINS;
+  const bool k_exact = k_binds && c_in[k0] == k;
+  bool p_binds = false, m_binds = false;
+  int m0 = BINS, m1 = BINS, from[4] = {0, BINS, BINS, BINS}, to[4] = {min(k0, BINS - 1), -1, -1, -1};       // runs of bins that are wanted
+  if (!whole) {
+    const double mk_hi = k_binds ? m_in[k0] : all, mk_lo = !k_binds || k_exact ? mk_hi : k0 > 0 ? m_in[k0 - 1] : 0.0;
+    int p0 = BINS, p1 = BINS;
+    if (set.p < 1.0) {
+      p0 = __syncthreads_count(bin && m < set.p * mk_lo - slack);
+      p1 = max(0, __syncthreads_count(bin && m_ex < set.p * mk_hi + slack) - 1);
+    }
+    if (set.m > 0.0 && set.m <= 1.0) {
+      const double off = fabs(line) * 1e-15 + 1e-6, at = first - line - PER_T * log(set.m);
+      m0 = (int)fmin(fmax(ceil(at - off), 0.0), (double)BINS);
+      m1 = (int)fmin(fmax(floor(at + 1.0 + off), 0.0), (double)BINS);
+      if (m1 >= BINS) m1 = m0 = BINS;        // (what weighs less is in no bin)
+    }
+    const int end = min(min(k0, p1), m1);
+    p_binds = p0 <= end && p0 < BINS;
+    m_binds = m0 <= end && m0 < BINS;
+    double lo = mk_lo, hi = mk_hi;
+    if (p_binds) { lo = fmin(lo, set.p * mk_lo - slack); hi = fmin(hi, m_in[min(p1, BINS - 1)]); }
+    if (m_binds) { lo = fmin(lo, m0 > 0 ? m_in[m0 - 1] : 0.0); hi = fmin(hi, m_in[m1]); }
+    lo = fmax(lo, 0.0);
+    const int d0 = __syncthreads_count(bin && m <= set.u * lo - slack), d1 = __syncthreads_count(bin && m_ex <= set.u * hi + slack) - 1;
+    from[0] = d0;
+    to[0] = min(d1, end);
+    if (p_binds) { from[1] = p0; to[1] = min(p1, end); }
+    if (m_binds) { from[2] = m0; to[2] = m1; }
+    if (k_binds && !k_exact && (k0 <= end || p_binds)) from[3] = to[3] = k0;
+  }
+  auto wanted = [&](int j) { return (j >= from[0] && j <= to[0]) || (j >= from[1] && j <= to[1]) || (j >= from[2] && j <= to[2]) || (j >= from[3] && j <= to[3]); };
+  const bool flag = bin && wanted(b);
+  int g = 0;
+  if (bin) {
+    const unsigned long long bal = __ballot(flag);
+    g = __popcll(bal & ((1ull << lane) - 1ull));
+    if (lane == 0) wave_s[wave] = __popcll(bal);
+  }
+  // the wanted runs as values: the least float of a run's last bin (of those that this slice has counted: 256 from its own largest on), the least above its first
+  if (b >= NT - 8) {
+    const int i = (b & 7) >> 1, above = b & 1, f = i == 0 ? from[0] : i == 1 ? from[1] : i == 2 ? from[2] : from[3], t = i == 0 ? to[0] : i == 1 ? to[1] : i == 2 ? to[2] : to[3];
+    const double floor_of = first - shift[p] - (BINS - 1);
+    float v;
+    if (flat || !(per > 0.0)) v = above ? NAN : f <= 0 && t >= 0 ? (flat ? top : -3.402823466e38f) : NAN;
+    else v = least_at(above ? first - f + 1.0 : fmax(first - t, floor_of), per);
+    bounds[i][above] = v;
+  }
+  __syncthreads();
+  if (p == 0 && bin) {
+    for (int w = 0; w < wave; ++w) g += wave_s[w];
+    RowSums& o = *s.sums;
+    o.mass[b] = m_ex;
+    o.count[b] = c - c_own;
+    o.slot[b] = flag ? (short)g : (short)-1;
+    if (b == 0)
+      o.said = RowSaid{all, c_all, wave_s[0] + wave_s[1] + wave_s[2] + wave_s[3], k_binds ? (k_exact ? 2 : 1) : 0, k0, m0, m1, p_binds, m_binds, whole, 0};
+  }
+  // this slice's: none where none of its bins are wanted
+  const int own = b - shift[p];
+  if (!__syncthreads_or(bin && flag && own >= 0 && s.bins[p * BINS + max(own, 0)] > 0ull)) return;
+  if constexpr (!EARLY) load_slice<NT, NE, VEC>(x, logits + (long)r * ld, base, V);
+  unsigned mask = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (from[i] <= to[i]) {
+      const float lo = bounds[i][0], hi = bounds[i][1];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) mask |= x[e] >= lo && !(x[e] >= hi) ? 1u << e : 0u;
+    }
+  int n = __popc(mask), at = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(at, o, 64); if (lane >= o) at += v; }
+  const int sum = __shfl(at, 63, 64);
+  if (sum > 0) {
+    int start = 0;
+    if (lane == 0) start = atomicAdd(&found, sum);
+    at += __shfl(start, 0, 64) - n;
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+      if (mask >> e & 1) {
+        if (at < SLICE_CAP) s.found[(long)p * SLICE_CAP + at] = ((unsigned long long)key_of(x[e]) << 32) | (unsigned)(0x7fffffff - index_of<NT, NE, VEC>(base, e));
+        ++at;
+      }
+  }
+  __syncthreads();
+  if (b == 0) s.heads[p].found = found;
+}
+
+// Largest first, `n` a power of two of 64 to 2 ST.  Two neighbours a thread: partners at most 64 places apart are in the same wave and change places by
+// shuffles, others through LDS.
+__device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
+  typedef unsigned long long u64;
+  const int i0 = 2 * threadIdx.x;
+  const bool on = i0 < n;
+  __syncthreads();
+  u64 a = on ? v[i0] : 0ull, b = on ? v[i0 + 1] : 0ull;
+  for (int k = 2; k <= n; k <<= 1) {
+    const bool down = (i0 & k) == 0;
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (j == 1) {
+        if ((a < b) == down) { const u64 t = a; a = b; b = t; }
+      } else {
+        u64 c, d;
+        if (j <= 64) {
+          c = __shfl_xor(a, j >> 1, 64);
+          d = __shfl_xor(b, j >> 1, 64);
+        } else {
+          __syncthreads();
+          if (on) { v[i0] = a; v[i0 + 1] = b; }
+          __syncthreads();
+          c = on ? v[i0 ^ j] : 0ull;
+          d = on ? v[(i0 ^ j) + 1] : 0ull;
+        }
+        const bool large = ((i0 & j) == 0) == down;        // of a pair the one in front takes the larger one, where it runs down
+        a = (a < c) == large ? c : a;
+        b = (b < d) == large ? d : b;
+      }
+    }
+  }
+  __syncthreads();
+  if (on) { v[i0] = a; v[i0 + 1] = b; }
+  __syncthreads();
+}
+// sums over the threads in front of each, and with it
+template <typename T> __device__ __forceinline__ T sum_upto(T v, T* room /* ST / 64 */) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) { const T x = __shfl_up(v, o, 64); if (lane >= o) v += x; }
+  __syncthreads();
+  if (lane == 63) room[wave] = v;
+  __syncthreads();
+  T w = lane < wave ? room[lane & (ST / 64 - 1)] : T(0);
+#pragma unroll
+  for (int o = ST / 128; o > 0; o >>= 1) w += __shfl_xor(w, o, 64);
+  return v + __shfl(w, 0, 64);
+}
+
+// a workgroup a row
+template <bool SMALL>
+__global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ tokens, float* __restrict__ probs, char* __restrict__ scratch, int P, int slice,
+                                                            const float* __restrict__ logits, long ld, int V, const float* __restrict__ uniforms,
+                                                            const float* __restrict__ temperature, const int* __restrict__ top_k, const float* __restrict__ top_p,
+                                                            const float* __restrict__ min_p) {
+  typedef unsigned long long u64;
+  __shared__ __attribute__((aligned(16))) u64 v[CAP], raw[CAP];    // tokens; whole masses up to and with each
+  __shared__ double front_m[CAP];                                  // mass and count in front of each bin
+  __shared__ int front_c[CAP], start[CAP];                         // where a bin's tokens start in v
+  __shared__ u64 wide[ST / 64];
+  __shared__ int narrow[ST / 64];
+  __shared__ short slot[BINS], bin_of[BINS];
+  __shared__ unsigned char want[CAP];
+  __shared__ SlowRoom room;
+  __shared__ int from[P_MAX + 1], got[4], ranks, taken;
+  __shared__ double masses;
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float* row = logits + (long)r * ld;
+  const RowSettings set = row_settings(r, V, temperature, top_k, top_p, min_p, uniforms);
+  const Scratch s = SMALL ? Scratch{} : scratch_of(scratch, r, P, slice);
+  float top = -INFINITY;
+  int first_at = 0, had = 0;
+  RowSaid said{};
+  if constexpr (!SMALL) said = s.sums->said;     // (asked for with the heads; a greedy row has none)
+  if constexpr (SMALL) {
+    u64 best = 0ull;
+    for (int i = tid; i < V; i += ST) {
+      const u64 k = ((u64)key_of(row[i]) << 32) | (unsigned)(0x7fffffff - i);
+      v[i] = k;
+      best = k > best ? k : best;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { const u64 k = __shfl_xor(best, o, 64); best = k > best ? k : best; }
+    if (lane == 0) wide[wave] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < ST / 64; ++w) best = wide[w] > best ? wide[w] : best;
+    __syncthreads();
+    top = of_key((unsigned)(best >> 32));
+    first_at = 0x7fffffff - (int)(best & 0xffffffffu);
+  } else {
+    const SliceHead h = lane < P ? s.heads[lane] : SliceHead{-INFINITY, 0, 0, 0};
+    top = wave_max(h.top);
+    const unsigned long long bal = __ballot(h.top == top);
+    first_at = __shfl(h.at, __ffsll(bal) - 1, 64);
+    had = h.found;
+  }
+  if (!(top > -INFINITY) || set.greedy) {
+    if (tid == 0) {
+      tokens[r] = top > -INFINITY ? first_at : -1;
+      if (probs) probs[r] = top > -INFINITY ? 1.f : 0.f;
+    }
+    return;
+  }
+  const double inv_t = 1.0 / set.t, per = PER_T / set.t, first = floor(line_of(top, per)), slack_of = 1e-11;
+  auto value = [](u64 t) { return of_key((unsigned)(t >> 32)); };
+  auto token_weight = [&](u64 t) { return (unsigned)(t >> 32) > KEY_NONE ? weight_at(value(t), top, inv_t) : 0.0; };
+  int n = V, slots = 1;
+  bool whole = true, p_binds = set.p < 1.0, m_binds = set.m > 0.0 && set.m <= 1.0;
+  const int k = set.m > 1.0 ? 1 : set.k;
+  int m0 = 0, m1 = BINS - 1, found = 0;
+  if constexpr (!SMALL) {
+    if (__ballot(had > slice / 4)) {
+      sample_slow(r, tokens, probs, row, V, set, top, room);
+      return;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(had, o, 64); if (lane >= o) had += x; }
+    if (wave == 0) {
+      if (lane < P) from[lane + 1] = had;
+      if (lane == 0) from[0] = 0;
+    }
+    __syncthreads();
+    n = found = from[P];
+    whole = said.whole;
+    if (!whole) {
+      p_binds = said.p_binds;
+      m_binds = said.m_binds;
+      m0 = said.m0;
+      m1 = said.m1;
+    }
+    slots = said.slots;
+    if (tid < BINS) {
+      slot[tid] = s.sums->slot[tid];
+      if (slot[tid] >= 0) bin_of[slot[tid]] = (short)tid;
+    }
+  }
+  const bool many = !SMALL && found > CAP;
+  // bins of the collected tokens: all in one (front of it nothing); those of collect; or `cut` in each of those
+  int cut = 1;
+  if (many) while (2 * cut * slots <= CAP && cut < 256) cut *= 2;
+  auto place = [&](u64 t) -> int {
+    if (SMALL || (whole && !many)) return 0;
+    const double l = floor(line_of(value(t), per) * cut), c = floor(l * (1.0 / cut));
+    const int j = max(0, min(BINS - 1, (int)(first - c)));
+    return many ? max(0, (int)slot[j]) * cut + (cut - 1 - (int)(l - c * cut)) : j;
+  };
+  auto collected = [&](int i) -> u64 {       // in memory, slice behind slice
+    int lo = 0, hi = P - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (from[mid + 1] > i) hi = mid;
+      else lo = mid + 1;
+    }
+    return s.found[(long)lo * (slice / 4) + i - from[lo]];
+  };
+  if (tid < 4) got[tid] = CAP;
+  if (tid == 0) taken = 0;
+  if (many) for (int i = tid; i < CAP; i += ST) { raw[i] = 0ull; start[i] = 0; }
+  __syncthreads();
+  // min-p's end: as many as weigh enough
+  int count_m = 0;
+  u64 mass_m = 0ull;
+  auto enough = [&](u64 t, double w) {
+    if (!m_binds || !(w >= set.m) || (unsigned)(t >> 32) <= KEY_NONE) return;
+    if (!SMALL && !whole) {
+      const int j = (int)(first - floor(line_of(value(t), per)));
+      if (j < m0 || j > m1) return;
+    }
+    ++count_m;
+    mass_m += fine_of(w);
+  };
+  if (many)
+    for (int i = tid; i < found; i += ST) {
+      const u64 t = collected(i);
+      const double w = token_weight(t);
+      enough(t, w);
+      const int b = place(t);
+      atomicAdd(&raw[b], fine_of(w));
+      atomicAdd(&start[b], 1);
+    }
+  else {
+    if constexpr (!SMALL) {
+      for (int i = tid; i < n; i += ST) v[i] = collected(i);
+      __syncthreads();
+    }
+    for (int i = tid; i < n; i += ST) enough(v[i], token_weight(v[i]));
+  }
+  double end_m = 0.0;
+  if (m_binds) {
+    mass_m = sum_upto(mass_m, wide);
+    count_m = sum_upto(count_m, narrow);
+    __syncthreads();
+    if (tid == ST - 1) { wide[0] = mass_m; narrow[0] = count_m; }
+    __syncthreads();
+    count_m = narrow[0];
+    end_m = (double)wide[0] * (1.0 / FINE_ONE);
+    if (!SMALL && !whole) { count_m += s.sums->count[m0]; end_m += s.sums->mass[m0]; }
+  }
+  __syncthreads();
+  int how_k = SMALL || whole ? (k < n ? 1 : 0) : said.k_binds, count = SMALL || whole ? n : said.count_all;
+  double mass = 0.0;                         // of everything, then of the first k
+  if (!SMALL && !whole) {
+    mass = said.all;
+    if (how_k == 2) {
+      count = k;
+      mass = said.k0 + 1 < BINS ? s.sums->mass[said.k0 + 1] : said.all;
+    }
+  }
+  if (many) {
+    // each bin's sums, from those in front of it; then which bins the ends may lie in, as collect does
+    const int b0 = 2 * tid;
+    const u64 q0 = raw[b0], q1 = raw[b0 + 1];
+    const int c0 = start[b0], c1 = start[b0 + 1];
+    const u64 qs = sum_upto(q0 + q1, wide);
+    const int cs = sum_upto(c0 + c1, narrow);
+    __syncthreads();
+    raw[b0] = qs - q0 - q1;
+    raw[b0 + 1] = qs - q1;
+    start[b0] = cs - c0 - c1;
+    start[b0 + 1] = cs - c1;
+    __syncthreads();
+    const int used = slots * cut;
+    double ex[2], in[2];
+    int c_in[2], c_ex[2];
+    bool is[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int b = b0 + e;
+      is[e] = b < used;
+      ex[e] = in[e] = 0.0;
+      c_ex[e] = c_in[e] = 0;
+      if (is[e]) {
+        const int z = b / cut * cut, j = bin_of[b / cut];
+        const u64 q = raw[b] - (whole ? 0ull : raw[z]);
+        ex[e] = (whole ? 0.0 : s.sums->mass[j]) + (double)q * (1.0 / FINE_ONE);
+        in[e] = (whole ? 0.0 : s.sums->mass[j]) + (double)(q + (e ? q1 : q0)) * (1.0 / FINE_ONE);
+        c_ex[e] = whole ? start[b] : s.sums->count[j] + start[b] - start[z];
+        c_in[e] = c_ex[e] + (e ? c1 : c0);
+      }
+      front_m[b] = ex[e];
+      front_c[b] = c_ex[e];
+    }
+    if (whole) {
+      if (tid == ST - 1) masses = (double)qs * (1.0 / FINE_ONE);
+      __syncthreads();
+      mass = masses;
+    }
+    const double slack = slack_of * mass;
+    auto before = [&](bool a, bool b) { const bool h[2] = {is[0] && a, is[1] && b}; return bins_with(h); };
+    const int k0 = how_k == 1 ? before(c_in[0] < k, c_in[1] < k) : used;
+    double lo = mass, hi = mass;
+    if (k0 < used) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) if (b0 + e == k0) { masses = in[e]; got[0] = c_in[e] == k ? 1 : 0; }
+      __syncthreads();
+      hi = masses;
+      if (got[0] == 1) {
+        how_k = 2;
+        count = k;
+        lo = mass = hi;
+      } else lo = front_m[k0];
+      __syncthreads();
+      if (tid == 0) got[0] = CAP;
+    }
+    int p0 = used, p1 = -1;
+    if (p_binds) {
+      p0 = before(in[0] < set.p * lo - slack, in[1] < set.p * lo - slack);
+      p1 = before(ex[0] < set.p * hi + slack, ex[1] < set.p * hi + slack) - 1;
+      p1 = max(p1, 0);
+      if (p0 < used) {
+        lo = fmin(lo, set.p * lo - slack);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 2; ++e) if (b0 + e == p1) masses = in[e];
+        __syncthreads();
+        hi = fmin(hi, masses);
+      }
+    }
+    if (m_binds) { lo = fmin(lo, end_m - slack); hi = fmin(hi, end_m + slack); }
+    lo = fmax(lo, 0.0);
+    const double ulo = set.u * lo - slack, uhi = set.u * hi + slack;
+    const int d0 = before(in[0] <= ulo, in[1] <= ulo), d1 = before(ex[0] <= uhi, ex[1] <= uhi) - 1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int b = b0 + e;
+      want[b] = is[e] && ((b >= p0 && b <= p1) || (b >= d0 && b <= d1) || (how_k == 1 && b == k0));
+    }
+    __syncthreads();
+    for (int i = tid; i < found; i += ST) {
+      const u64 t = collected(i);
+      if (want[place(t)]) {
+        const int at = atomicAdd(&taken, 1);
+        if (at < CAP) v[at] = t;
+      }
+    }
+    __syncthreads();
+    n = taken;
+    if (n > CAP) {
+      sample_slow(r, tokens, probs, row, V, set, top, room);
+      return;
+    }
+  } else if (!SMALL && !whole) {
+    if (tid < BINS) { front_m[tid] = s.sums->mass[tid]; front_c[tid] = s.sums->count[tid]; }
+  } else if (tid == 0) { front_m[0] = 0.0; front_c[0] = 0; }
+  int size = 64;
+  while (size < n) size <<= 1;
+  for (int i = n + tid; i < size; i += ST) v[i] = 0ull;
+  sort_down(v, size);
+  // mass up to and with each token, and its rank
+  const int e0 = 2 * tid;
+  u64 q[2] = {0ull, 0ull};
+  double w[2] = {0.0, 0.0}, in[2] = {0.0, 0.0};
+  int rank[2] = {1 << 30, 1 << 30}, bin[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (e0 + e < n) {
+      w[e] = token_weight(v[e0 + e]);
+      q[e] = fine_of(w[e]);
+      bin[e] = place(v[e0 + e]);
+      if (e0 + e == 0 || place(v[e0 + e - 1]) != bin[e]) start[bin[e]] = e0 + e;
+    }
+  const u64 sum = sum_upto(q[0] + q[1], wide);
+  raw[e0] = sum - q[1];
+  raw[e0 + 1] = sum;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (e0 + e < n) {
+      const int at = start[bin[e]];
+      in[e] = front_m[bin[e]] + (double)(raw[e0 + e] - (at > 0 ? raw[at - 1] : 0ull)) * (1.0 / FINE_ONE);
+      rank[e] = front_c[bin[e]] + e0 + e - at;
+    }
+  // the ends: what is kept is the first `count`, of mass `mass`
+  if ((SMALL || whole) && !many) {
+    if (e0 <= n - 1 && n - 1 <= e0 + 1) masses = in[n - 1 - e0];
+    __syncthreads();
+    mass = masses;
+  }
+  __syncthreads();
+  if (how_k == 1) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) if (rank[e] == k - 1) { got[0] = 0; masses = in[e]; }
+  }
+  __syncthreads();
+  if (how_k == 1 && got[0] == 0) { count = k; mass = masses; }
+  const double limit = fmax(set.p, 0.0) * mass;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (e0 + e < n && p_binds && in[e] >= limit) atomicMin(&got[1], e0 + e);
+  __syncthreads();
+  const int kp = got[1];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) if (e0 + e == kp) { ranks = rank[e] + 1; masses = in[e]; }
+  __syncthreads();
+  if (m_binds && count_m < count) { count = count_m; mass = end_m; }
+  if (p_binds && kp < CAP && ranks < count) { count = ranks; mass = masses; }
+  if (count < 1) { count = 1; mass = 1.0; }
+  // the draw: the first over the goal, the last kept one where the sums' rounding leaves none
+  const double goal = set.u * mass;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (e0 + e < n && q[e] && rank[e] < count && in[e] > goal) atomicMin(&got[2], e0 + e);
+  __syncthreads();
+  int at = got[2];
+  if (at >= CAP) {
+    if (tid == 0) got[3] = -1;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (e0 + e < n && q[e] && rank[e] < count) atomicMax(&got[3], e0 + e);
+    __syncthreads();
+    at = max(got[3], 0);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (e0 + e == at) {
+      tokens[r] = 0x7fffffff - (int)(v[at] & 0xffffffffu);
+      if (probs) probs[r] = (float)(w[e] / mass);
+    }
+}
+
+// slices of 32768 values where rows fill the chip by themselves, of 8192 where they do not (one row of 128256: 16 workgroups instead of 4)
+static int slice_values(int rows, int V) { return rows >= 64 ? 32768 : 8192; }
+static int slices_of(int rows, int V) { const int n = slice_values(rows, V); return (V + n - 1) / n; }
+
+extern "C" long umb_sample_requests_bytes(int rows, int V) {
+  if (rows < 1 || V < 1 || V > SAMPLE_VMAX) return 0;
+  return V <= SMALL_V ? 16 : rows * row_bytes(slices_of(rows, V), slice_values(rows, V));
+}
 
 extern "C" int umb_sample_requests(int* tokens, float* probs, const float* logits, long ld, int rows, int V, const float* uniforms,
                                    const float* temperature, const int* top_k, const float* top_p, const float* min_p, void* scratch, long scratch_bytes,
@@ -206,7 +922,31 @@ extern "C" int umb_sample_requests(int* tokens, float* probs, const float* logit
   if (!tokens || !logits || !uniforms || !scratch || rows < 1 || V < 1 || V > SAMPLE_VMAX || ld < V || (uintptr_t)scratch % 16 ||
       scratch_bytes < umb_sample_requests_bytes(rows, V))
     return UMB_EINVAL;
-  hipLaunchKernelGGL(sample_requests_kernel, dim3(rows), dim3(ST), 0, st, tokens, probs, logits, ld, V, uniforms, temperature, top_k, top_p, min_p);
-  UMB_LAUNCH_CHECK();
+  if (V <= SMALL_V) {
+    hipLaunchKernelGGL((sample_resolve_kernel<true>), dim3(rows), dim3(ST), 0, st, tokens, probs, (char*)nullptr, 0, 0, logits, ld, V, uniforms, temperature, top_k, top_p,
+                       min_p);
+    UMB_LAUNCH_CHECK();
+    return UMB_OK;
+  }
+  const int P = slices_of(rows, V), slice = slice_values(rows, V);
+  const bool vec = (uintptr_t)logits % 16 == 0 && ld % 4 == 0, large = slice == 32768;
+  char* room = static_cast<char*>(scratch);
+  for (int r0 = 0; r0 < rows; r0 += 65535) {                 // (a grid's rows)
+    const int n = rows - r0 < 65535 ? rows - r0 : 65535;
+    char* const sc = room + r0 * row_bytes(P, slice);
+    const float* const x = logits + r0 * ld;
+    auto at = [&](auto* p) { return p ? p + r0 : p; };
+#define SLICES(NT, NE, VEC)                                                                                                                                 \
+  hipLaunchKernelGGL((sample_slices_kernel<NT, NE, VEC>), dim3(P, n), dim3(NT), 0, st, sc, x, ld, V, at(temperature), at(top_k));                                       \
+  hipLaunchKernelGGL((sample_collect_kernel<NT, NE, VEC>), dim3(P, n), dim3(NT), 0, st, sc, x, ld, V, at(uniforms), at(temperature), at(top_k), at(top_p), at(min_p))
+    if (large && vec) { SLICES(1024, 32, true); }
+    else if (large) { SLICES(1024, 32, false); }
+    else if (vec) { SLICES(512, 16, true); }
+    else { SLICES(512, 16, false); }
+#undef SLICES
+    hipLaunchKernelGGL((sample_resolve_kernel<false>), dim3(n), dim3(ST), 0, st, at(tokens), at(probs), sc, P, slice, x, ld, V, at(uniforms), at(temperature), at(top_k),
+                       at(top_p), at(min_p));
+    UMB_LAUNCH_CHECK();
+  }
   return UMB_OK;
 }
