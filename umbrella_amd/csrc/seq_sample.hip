@@ -192,17 +192,24 @@ constexpr double MAGIC = 4503599627370496.0;                     // 2^52: added 
 constexpr double BIN_ONE = 4294967296.0;                         // a bin's masses, in 2^-32 of its middle's weight: 48 bits for 2^15 of them, 16 above for their number
 constexpr double FINE_ONE = 70368744177664.0;                    // 2^46, of the row's largest weight
 
-// e^(f / 8) of -0.5 <= f <= 0.5: Taylor's sum to the sixth power, good to 1e-12 of it
-__device__ __forceinline__ double exp_bin(double f) {
-  constexpr double c = 1.0 / PER_T;
-  double p = c * c * c * c * c * c / 720.0;
-  p = fma(p, f, c * c * c * c * c / 120.0);
-  p = fma(p, f, c * c * c * c / 24.0);
-  p = fma(p, f, c * c * c / 6.0);
-  p = fma(p, f, c * c / 2.0);
-  p = fma(p, f, c);
-  return fma(p, f, 1.0);
-}
+// e^((f - 1/2) / 8) of 0 <= f < 1 in whole numbers of 1 / BIN_ONE: the polynomial of degree 5 that meets it in the six Chebyshev points, good to 2.8e-12 of it
+// (mean 7e-14), rounded by the addition of 2^52.  The coefficients are held in registers: as literals each costs two moves an element.
+struct BinExp {
+  double c[6];
+  __device__ __forceinline__ BinExp() {
+    const double k[6] = {0.9394130628109114, 0.11742663303627268, 0.007339162402444743, 0.00030580767554919385, 9.5386414386407e-06, 2.54348632176618e-07};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) c[i] = k[i] * BIN_ONE + (i == 0 ? MAGIC : 0.0);
+#pragma unroll
+    for (int i = 0; i < 6; ++i) asm volatile("" : "+v"(c[i]));
+  }
+  __device__ __forceinline__ unsigned long long operator()(double f) const {
+    double p = c[5];
+#pragma unroll
+    for (int i = 4; i >= 0; --i) p = fma(p, f, c[i]);
+    return (unsigned long long)__double_as_longlong(p) & 0x7ffffffffffffull;
+  }
+};
 // e^d of -40 < d <= 0.1 to some 2e-15 of it (a power of two times Taylor's sum to the 12th power of a rest of at most 0.347), 0 below
 __device__ __forceinline__ double exp_down(double d) {
   if (!(d > -40.0)) return 0.0;
@@ -334,22 +341,25 @@ __global__ __launch_bounds__(NT) void sample_slices_kernel(char* __restrict__ sc
   const double per = PER_T / (double)t, first = floor(line_of(top, per));
   const int k = top_k ? top_k[r] : 0;
   unsigned long long* const mine = bins + (threadIdx.x & (COPIES - 1));
-  auto count = [&](int j, unsigned long long v) __attribute__((always_inline)) { atomicAdd(mine + COPIES * j, v); };
   if (top == INFINITY || !(fabs((double)top * per) < LATTICE)) {   // its equals alone count
 #pragma unroll
-    for (int e = 0; e < NE; ++e) if (x[e] == top) count(0, 1ull << 48);
+    for (int e = 0; e < NE; ++e) if (x[e] == top) atomicAdd(mine, 1ull << 48);
   } else if (k >= 1 && k <= K_COUNT) {
     // (-inf, and what the lattice does not reach, are far below)
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
       const double j = first - floor((double)x[e] * per);
-      if (j < BINS) atomicAdd(reinterpret_cast<unsigned*>(mine + COPIES * (int)j) + 1, 1u << 16);
+      const int at = COPIES * (int)j;
+      if (j < BINS) atomicAdd(reinterpret_cast<unsigned*>(mine + at) + 1, 1u << 16);
     }
   } else {
+    const BinExp weight;
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
+    for (int e = 0; e < NE; ++e) {           // (worked out for all, so that elements run side by side)
       const double l = (double)x[e] * per, f = floor(l), j = first - f;
-      if (j < BINS) count((int)j, (1ull << 48) + ((unsigned long long)__double_as_longlong(fma(exp_bin(l - f - 0.5), BIN_ONE, MAGIC)) & 0x7ffffffffffffull));
+      const int at = COPIES * (int)j;
+      const unsigned long long v = (1ull << 48) + weight(l - f);
+      if (j < BINS) atomicAdd(mine + at, v);
     }
   }
   __syncthreads();
@@ -378,6 +388,8 @@ __global__ __launch_bounds__(NT) void sample_collect_kernel(char* __restrict__ s
   __shared__ double m_in[BINS], wave_m[4];
   __shared__ int shift[P_MAX], c_in[BINS], wave_c[4], wave_s[4], found;
   __shared__ float bounds[4][2];
+  __shared__ unsigned long long other_q[NT / BINS - 1][BINS];
+  __shared__ int other_c[NT / BINS - 1][BINS];
   const int r = blockIdx.y, P = gridDim.x, p = blockIdx.x, b = threadIdx.x, lane = b & 63, wave = b >> 6;
   const RowSettings set = row_settings(r, V, temperature, top_k, top_p, min_p, uniforms);
   if (set.greedy) return;
@@ -397,19 +409,24 @@ __global__ __launch_bounds__(NT) void sample_collect_kernel(char* __restrict__ s
   }
   if (b == 0) found = 0;
   __syncthreads();
-  int c = 0;
+  // the slices' bins, every GROUPS-th by 256 threads each
+  constexpr int GROUPS = NT / BINS;
   unsigned long long q = 0ull;
-  if (bin) {
+  int c = 0;
 #pragma unroll 8
-    for (int i = 0; i < P; ++i) {
-      const int k = b - shift[i];
-      const unsigned long long v = s.bins[i * BINS + max(k, 0)];
-      if (k >= 0) {
-        c += (int)(v >> 48);
-        q += v & 0xffffffffffffull;
-      }
+  for (int i = b / BINS; i < P; i += GROUPS) {
+    const int k = b % BINS - shift[i];
+    const unsigned long long v = s.bins[i * BINS + max(k, 0)];
+    if (k >= 0) {
+      c += (int)(v >> 48);
+      q += v & 0xffffffffffffull;
     }
   }
+  if (!bin) { other_q[b / BINS - 1][b % BINS] = q; other_c[b / BINS - 1][b % BINS] = c; }
+  __syncthreads();
+  if (bin)
+#pragma unroll
+    for (int i = 0; i < GROUPS - 1; ++i) { q += other_q[i][b]; c += other_c[i][b]; }
   // a bin's middle beside the largest; beside an infinite one, or one beyond the lattice, only its equals count
   const bool flat = top == INFINITY || !(fabs((double)top * per) < LATTICE);
   double m = !bin ? 0.0 : flat ? (b == 0 ? (double)c : 0.0) : (double)q * (1.0 / BIN_ONE) * exp_down((first - b + 0.5 - line) * (1.0 / PER_T));
@@ -529,7 +546,7 @@ __global__ __launch_bounds__(NT) void sample_collect_kernel(char* __restrict__ s
 __device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
   typedef unsigned long long u64;
   const int i0 = 2 * threadIdx.x;
-  const bool on = i0 < n;
+  const bool on = i0 < n, busy = (i0 & ~127) < n;            // (a wave that has none of them leaves the others LDS's time)
   __syncthreads();
   u64 a = on ? v[i0] : 0ull, b = on ? v[i0 + 1] : 0ull;
   for (int k = 2; k <= n; k <<= 1) {
@@ -537,7 +554,7 @@ __device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
     for (int j = k >> 1; j > 0; j >>= 1) {
       if (j == 1) {
         if ((a < b) == down) { const u64 t = a; a = b; b = t; }
-      } else {
+      } else if (busy || j > 64) {
         u64 c, d;
         if (j <= 64) {
           c = __shfl_xor(a, j >> 1, 64);
@@ -560,8 +577,9 @@ __device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
   __syncthreads();
 }
 // sums over the threads in front of each, and with it
-template <typename T> __device__ __forceinline__ T sum_upto(T v, T* room /* ST / 64 */) {
+template <typename T> __device__ __forceinline__ T sum_upto(T v, T* room /* ST / 64 */, bool busy = true) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (busy)                                  // (a wave of zeros has no sums to form)
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) { const T x = __shfl_up(v, o, 64); if (lane >= o) v += x; }
   __syncthreads();
@@ -588,7 +606,8 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   __shared__ short slot[BINS], bin_of[BINS];
   __shared__ unsigned char want[CAP];
   __shared__ SlowRoom room;
-  __shared__ int from[P_MAX + 1], got[4], ranks, taken;
+  __shared__ int from[P_MAX + 1], got[4], ranks, taken, sum_c;
+  __shared__ u64 sum_m;
   __shared__ double masses;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* row = logits + (long)r * ld;
@@ -671,17 +690,25 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     const int j = max(0, min(BINS - 1, (int)(first - c)));
     return many ? max(0, (int)slot[j]) * cut + (cut - 1 - (int)(l - c * cut)) : j;
   };
-  auto collected = [&](int i) -> u64 {       // in memory, slice behind slice
-    int lo = 0, hi = P - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (from[mid + 1] > i) hi = mid;
-      else lo = mid + 1;
+  // f of each collected token, slice behind slice in memory; four loads of a thread in flight
+  auto each = [&](auto f) {
+    int at = 0;
+    for (int i0 = tid; i0 < found; i0 += 4 * ST) {
+      u64 t[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + e * ST;
+        if (i < found) {
+          while (from[at + 1] <= i) ++at;
+          t[e] = s.found[(long)at * (slice / 4) + i - from[at]];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (i0 + e * ST < found) f(i0 + e * ST, t[e]);
     }
-    return s.found[(long)lo * (slice / 4) + i - from[lo]];
   };
   if (tid < 4) got[tid] = CAP;
-  if (tid == 0) taken = 0;
+  if (tid == 0) { taken = 0; sum_c = 0; sum_m = 0ull; }
   if (many) for (int i = tid; i < CAP; i += ST) { raw[i] = 0ull; start[i] = 0; }
   __syncthreads();
   // min-p's end: as many as weigh enough
@@ -697,30 +724,30 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     mass_m += fine_of(w);
   };
   if (many)
-    for (int i = tid; i < found; i += ST) {
-      const u64 t = collected(i);
+    each([&](int, u64 t) {
       const double w = token_weight(t);
       enough(t, w);
       const int b = place(t);
       atomicAdd(&raw[b], fine_of(w));
       atomicAdd(&start[b], 1);
-    }
+    });
   else {
     if constexpr (!SMALL) {
-      for (int i = tid; i < n; i += ST) v[i] = collected(i);
+      each([&](int i, u64 t) { v[i] = t; });
       __syncthreads();
     }
     for (int i = tid; i < n; i += ST) enough(v[i], token_weight(v[i]));
   }
   double end_m = 0.0;
   if (m_binds) {
-    mass_m = sum_upto(mass_m, wide);
-    count_m = sum_upto(count_m, narrow);
+    if (__ballot(count_m > 0)) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) { mass_m += __shfl_xor(mass_m, o, 64); count_m += __shfl_xor(count_m, o, 64); }
+      if (lane == 0) { atomicAdd(&sum_m, mass_m); atomicAdd(&sum_c, count_m); }
+    }
     __syncthreads();
-    if (tid == ST - 1) { wide[0] = mass_m; narrow[0] = count_m; }
-    __syncthreads();
-    count_m = narrow[0];
-    end_m = (double)wide[0] * (1.0 / FINE_ONE);
+    count_m = sum_c;
+    end_m = (double)sum_m * (1.0 / FINE_ONE);
     if (!SMALL && !whole) { count_m += s.sums->count[m0]; end_m += s.sums->mass[m0]; }
   }
   __syncthreads();
@@ -814,13 +841,12 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       want[b] = is[e] && ((b >= p0 && b <= p1) || (b >= d0 && b <= d1) || (how_k == 1 && b == k0));
     }
     __syncthreads();
-    for (int i = tid; i < found; i += ST) {
-      const u64 t = collected(i);
+    each([&](int, u64 t) {
       if (want[place(t)]) {
         const int at = atomicAdd(&taken, 1);
         if (at < CAP) v[at] = t;
       }
-    }
+    });
     __syncthreads();
     n = taken;
     if (n > CAP) {
@@ -847,7 +873,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       bin[e] = place(v[e0 + e]);
       if (e0 + e == 0 || place(v[e0 + e - 1]) != bin[e]) start[bin[e]] = e0 + e;
     }
-  const u64 sum = sum_upto(q[0] + q[1], wide);
+  const u64 sum = sum_upto(q[0] + q[1], wide, 128 * wave < n);
   raw[e0] = sum - q[1];
   raw[e0 + 1] = sum;
   __syncthreads();
