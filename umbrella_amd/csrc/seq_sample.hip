@@ -8,8 +8,8 @@
 // any order puts it but for some 1e-12 of the mass.  (In 32 bits a flat row of 128256 values has thousands of borders that the sum's order moves.)
 //
 // Nothing is sorted but what stands next to a border.  Three launches:
-//   slices   a row in slices, each read once into registers: its largest, and counts and masses of bins an eighth of T wide, 256 below the largest (what is
-//            further down weighs less than 2^-46 of the row).  Bins lie on one lattice, floor(8 x / T), and masses are relative to their bin's middle, so
+//   slices   a row in slices, each read once into registers: its largest, and counts and masses of bins T / 32 wide, 1024 below the largest (what is
+//            further down weighs less than 2^-46 of the row).  Bins lie on one lattice, floor(32 x / T), and masses are relative to their bin's middle, so
 //            that slices' add up as whole numbers, count and mass in one 64-bit atomic
 //   collect  the row's bins, summed up from the top, say which bins hold the k-th value, the ends of top-p and min-p and the token drawn (intervals, since
 //            the mass behind p and u is known to a bin only); their tokens are collected, from slices that have any.  A row of a small k has counts alone, and
@@ -186,27 +186,27 @@ __device__ __attribute__((noinline)) void sample_slow(int r, int* __restrict__ t
 }
 
 // ------------------------------------------------------------------ bins
-constexpr int BINS = 256, SMALL_V = 2048, CAP = 2048, K_COUNT = 1024, P_MAX = 64;
-constexpr double PER_T = 8.0, LATTICE = 1099511627776.0;         // bins a T; beyond 2^40 neighbouring floats are 2^16 bins apart and more
+constexpr int BINS = 1024, SMALL_V = 2048, CAP = 2048, K_COUNT = 1024, P_MAX = 64;
+constexpr double PER_T = 32.0, LATTICE = 1099511627776.0;         // bins a T; beyond 2^40 neighbouring floats are 2^16 bins apart and more
 constexpr double MAGIC = 4503599627370496.0;                     // 2^52: added to a number below 2^51, it leaves the nearest whole number in the low bits
 constexpr double BIN_ONE = 4294967296.0;                         // a bin's masses, in 2^-32 of its middle's weight: 48 bits for 2^15 of them, 16 above for their number
 constexpr double FINE_ONE = 70368744177664.0;                    // 2^46, of the row's largest weight
 
-// e^((f - 1/2) / 8) of 0 <= f < 1 in whole numbers of 1 / BIN_ONE: the polynomial of degree 5 that meets it in the six Chebyshev points, good to 2.8e-12 of it
-// (mean 7e-14), rounded by the addition of 2^52.  The coefficients are held in registers: as literals each costs two moves an element.
+// e^((f - 1/2) / 32) of 0 <= f < 1 in whole numbers of 1 / BIN_ONE: the polynomial of degree 4 that meets it in the five Chebyshev points, good to 5e-13 of it,
+// rounded by the addition of 2^52.  The coefficients are held in registers: as literals each costs two moves an element.
 struct BinExp {
-  double c[6];
+  double c[5];
   __device__ __forceinline__ BinExp() {
-    const double k[6] = {0.9394130628109114, 0.11742663303627268, 0.007339162402444743, 0.00030580767554919385, 9.5386414386407e-06, 2.54348632176618e-07};
+    const double k[5] = {0.9844964370058922, 0.03076551363223118, 0.0004807113442785956, 5.006866963355461e-06, 3.97368340715931e-08};
 #pragma unroll
-    for (int i = 0; i < 6; ++i) c[i] = k[i] * BIN_ONE + (i == 0 ? MAGIC : 0.0);
+    for (int i = 0; i < 5; ++i) c[i] = k[i] * BIN_ONE + (i == 0 ? MAGIC : 0.0);
 #pragma unroll
-    for (int i = 0; i < 6; ++i) asm volatile("" : "+v"(c[i]));
+    for (int i = 0; i < 5; ++i) asm volatile("" : "+v"(c[i]));
   }
   __device__ __forceinline__ unsigned long long operator()(double f) const {
-    double p = c[5];
+    double p = c[4];
 #pragma unroll
-    for (int i = 4; i >= 0; --i) p = fma(p, f, c[i]);
+    for (int i = 3; i >= 0; --i) p = fma(p, f, c[i]);
     return (unsigned long long)__double_as_longlong(p) & 0x7ffffffffffffull;
   }
 };
@@ -254,7 +254,7 @@ __device__ __forceinline__ float least_at(double goal, double per) {
   return of_key(k);
 }
 
-struct SliceHead { float top; int at, found, pad; };
+struct SliceHead { float top; int at, pad[2]; };
 // what collect leaves for resolve; `mass` and `count`: in front of each bin
 struct RowSaid {
   double all;
@@ -268,15 +268,29 @@ struct RowSums {
   RowSaid said;
 };
 static_assert(sizeof(RowSums) % 16 == 0 && sizeof(RowSaid) % 16 == 0);
-struct Scratch { SliceHead* heads; unsigned long long *bins, *found; RowSums* sums; };
-__host__ __device__ __forceinline__ long row_bytes(int P, int slice) { return (long)P * (16 + BINS * 8 + slice / 4 * 8) + (long)sizeof(RowSums); }
-__device__ __forceinline__ Scratch scratch_of(char* base, int row, int P, int slice) {
-  char* p = base + row * row_bytes(P, slice);
+// How a row is cut: slices of `slice` values (P), which the first launch counts; chunks of `chunk` values, every Q-th of which the second launch's block q looks
+// through, with room for a quarter of them.  Few rows: as many workgroups as there are pieces of 8192; many: larger pieces, and as many workgroups as stay
+// resident, since each adds up its row's bins first.
+struct Cut { int slice, P, chunk, Q, cap; };
+static Cut cut_of(int rows, int V) {
+  const bool few = (long)rows * ((V + 8191) / 8192) <= 512;
+  Cut c;
+  c.slice = c.chunk = few ? 8192 : 16384;
+  c.P = (V + c.slice - 1) / c.slice;
+  c.Q = few ? c.P : std::max(1, std::min(c.P, 512 / rows));
+  c.cap = (c.P + c.Q - 1) / c.Q * (c.chunk / 4);
+  return c;
+}
+struct Scratch { SliceHead* heads; unsigned long long *bins, *found; int* taken; RowSums* sums; };
+__host__ __device__ __forceinline__ long row_bytes(const Cut& c) { return (long)c.P * (16 + BINS * 8) + (long)c.Q * c.cap * 8 + P_MAX * 4 + (long)sizeof(RowSums); }
+__device__ __forceinline__ Scratch scratch_of(char* base, int row, const Cut& c) {
+  char* p = base + row * row_bytes(c);
   Scratch s;
   s.bins = reinterpret_cast<unsigned long long*>(p);
-  s.found = s.bins + (long)P * BINS;
-  s.sums = reinterpret_cast<RowSums*>(s.found + (long)P * (slice / 4));
+  s.found = s.bins + (long)c.P * BINS;
+  s.sums = reinterpret_cast<RowSums*>(s.found + (long)c.Q * c.cap);
   s.heads = reinterpret_cast<SliceHead*>(s.sums + 1);
+  s.taken = reinterpret_cast<int*>(s.heads + c.P);
   return s;
 }
 
@@ -310,16 +324,15 @@ template <int NT, int NE, bool VEC> __device__ __forceinline__ void load_slice(f
 
 // grid (slices, rows)
 template <int NT, int NE, bool VEC>
-__global__ __launch_bounds__(NT) void sample_slices_kernel(char* __restrict__ scratch, const float* __restrict__ logits, long ld, int V,
+__global__ __launch_bounds__(NT) void sample_slices_kernel(char* __restrict__ scratch, Cut cut, const float* __restrict__ logits, long ld, int V,
                                                            const float* __restrict__ temperature, const int* __restrict__ top_k) {
-  constexpr int COPIES = 4;                  // of each bin, by lane: a row's values crowd in a few dozen bins
-  __shared__ unsigned long long bins[COPIES * BINS];
+  __shared__ unsigned long long bins[BINS];
   __shared__ float tops[NT / 64];
   __shared__ int at;
-  const int r = blockIdx.y, P = gridDim.x, p = blockIdx.x, base = p * NT * NE, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = blockIdx.y, p = blockIdx.x, base = p * NT * NE, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float x[NE];
   load_slice<NT, NE, VEC>(x, logits + (long)r * ld, base, V);
-  for (int i = threadIdx.x; i < COPIES * BINS; i += NT) bins[i] = 0ull;
+  for (int i = threadIdx.x; i < BINS; i += NT) bins[i] = 0ull;
   if (threadIdx.x == 0) at = 0x7fffffff;
   float top = -INFINITY;
 #pragma unroll
@@ -329,46 +342,55 @@ __global__ __launch_bounds__(NT) void sample_slices_kernel(char* __restrict__ sc
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) top = fmaxf(top, tops[w]);
-  const Scratch s = scratch_of(scratch, r, P, NT * NE);
+  const Scratch s = scratch_of(scratch, r, cut);
   const float t = temperature ? temperature[r] : 1.f;
   if (!(t > 0.f)) {                          // the first of the largest
 #pragma unroll
     for (int e = 0; e < NE; ++e) if (x[e] == top) atomicMin(&at, index_of<NT, NE, VEC>(base, e));
     __syncthreads();
   }
-  if (threadIdx.x == 0) s.heads[p] = SliceHead{top, at, 0, 0};
+  if (threadIdx.x == 0) s.heads[p] = SliceHead{top, at, {0, 0}};
   if (!(top > -INFINITY) || !(t > 0.f)) return;
   const double per = PER_T / (double)t, first = floor(line_of(top, per));
   const int k = top_k ? top_k[r] : 0;
-  unsigned long long* const mine = bins + (threadIdx.x & (COPIES - 1));
   if (top == INFINITY || !(fabs((double)top * per) < LATTICE)) {   // its equals alone count
 #pragma unroll
-    for (int e = 0; e < NE; ++e) if (x[e] == top) atomicAdd(mine, 1ull << 48);
+    for (int e = 0; e < NE; ++e) if (x[e] == top) atomicAdd(bins, 1ull << 48);
   } else if (k >= 1 && k <= K_COUNT) {
     // (-inf, and what the lattice does not reach, are far below)
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
       const double j = first - floor((double)x[e] * per);
-      const int at = COPIES * (int)j;
-      if (j < BINS) atomicAdd(reinterpret_cast<unsigned*>(mine + at) + 1, 1u << 16);
+      const int at = (int)j;
+      if (j < BINS) atomicAdd(reinterpret_cast<unsigned*>(bins + at) + 1, 1u << 16);
     }
   } else {
     const BinExp weight;
 #pragma unroll
     for (int e = 0; e < NE; ++e) {           // (worked out for all, so that elements run side by side)
       const double l = (double)x[e] * per, f = floor(l), j = first - f;
-      const int at = COPIES * (int)j;
+      const int at = (int)j;
       const unsigned long long v = (1ull << 48) + weight(l - f);
-      if (j < BINS) atomicAdd(mine + at, v);
+      if (j < BINS) atomicAdd(bins + at, v);
     }
   }
   __syncthreads();
-  if (threadIdx.x < BINS) {
-    unsigned long long sum = 0ull;
+  for (int i = threadIdx.x; i < BINS; i += NT) s.bins[p * BINS + i] = bins[i];
+}
+
+// sums over the threads in front of each, and with it, of a workgroup of NT; `busy` false: this wave's are zeros
+template <int NT, typename T> __device__ __forceinline__ T sum_upto(T v, T* room /* NT / 64 */, bool busy = true) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (busy)
 #pragma unroll
-    for (int i = 0; i < COPIES; ++i) sum += bins[COPIES * threadIdx.x + i];
-    s.bins[p * BINS + threadIdx.x] = sum;
-  }
+    for (int o = 1; o < 64; o <<= 1) { const T x = __shfl_up(v, o, 64); if (lane >= o) v += x; }
+  __syncthreads();
+  if (lane == 63) room[wave] = v;
+  __syncthreads();
+  T w = lane < wave ? room[lane & (NT / 64 - 1)] : T(0);
+#pragma unroll
+  for (int o = NT / 128; o > 0; o >>= 1) w += __shfl_xor(w, o, 64);
+  return v + __shfl(w, 0, 64);
 }
 
 // how many of `n` bins in a row, NB a thread, have what holds for the first of them and not for the rest
@@ -379,29 +401,24 @@ template <int NB> __device__ __forceinline__ int bins_with(const bool (&holds)[N
   return n;
 }
 
-// grid (slices, rows)
-template <int NT, int NE, bool VEC>
-__global__ __launch_bounds__(NT) void sample_collect_kernel(char* __restrict__ scratch, const float* __restrict__ logits, long ld, int V, const float* __restrict__ uniforms,
-                                                            const float* __restrict__ temperature, const int* __restrict__ top_k, const float* __restrict__ top_p,
-                                                            const float* __restrict__ min_p) {
-  constexpr int SLICE_CAP = NT * NE / 4;
-  __shared__ double m_in[BINS], wave_m[4];
-  __shared__ int shift[P_MAX], c_in[BINS], wave_c[4], wave_s[4], found;
+// grid (Q, rows); a thread a bin
+template <int NE, bool VEC>
+__global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restrict__ scratch, Cut cut, const float* __restrict__ logits, long ld, int V,
+                                                              const float* __restrict__ uniforms, const float* __restrict__ temperature, const int* __restrict__ top_k,
+                                                              const float* __restrict__ top_p, const float* __restrict__ min_p) {
+  constexpr int NT = BINS;
+  __shared__ double m_in[BINS], wave_m[NT / 64];
+  __shared__ int shift[P_MAX], c_in[BINS], wave_c[NT / 64], found;
   __shared__ float bounds[4][2];
-  __shared__ unsigned long long other_q[NT / BINS - 1][BINS];
-  __shared__ int other_c[NT / BINS - 1][BINS];
-  const int r = blockIdx.y, P = gridDim.x, p = blockIdx.x, b = threadIdx.x, lane = b & 63, wave = b >> 6;
+  const int r = blockIdx.y, P = cut.P, b = threadIdx.x, lane = b & 63;
+  int p = blockIdx.x;                        // chunk
   const RowSettings set = row_settings(r, V, temperature, top_k, top_p, min_p, uniforms);
   if (set.greedy) return;
-  const Scratch s = scratch_of(scratch, r, P, NT * NE);
-  // few rows wait for their loads one after the other: the slice is asked for early, wanted or not
-  constexpr bool EARLY = NE <= 16;
-  float x[NE];
-  const int base = p * NT * NE;
-  if constexpr (EARLY) load_slice<NT, NE, VEC>(x, logits + (long)r * ld, base, V);
+  const Scratch s = scratch_of(scratch, r, cut);
+  float x[NE];                               // (asked for early: what comes in between is latency)
+  load_slice<NT, NE, VEC>(x, logits + (long)r * ld, p * NT * NE, V);
   const float head = lane < P ? s.heads[lane].top : -INFINITY, top = wave_max(head);
   if (!(top > -INFINITY)) return;
-  const bool bin = b < BINS;
   const double per = PER_T / set.t, line = line_of(top, per), first = floor(line);
   if (b < P) {
     const double d = first - floor(line_of(head, per));
@@ -409,50 +426,32 @@ __global__ __launch_bounds__(NT) void sample_collect_kernel(char* __restrict__ s
   }
   if (b == 0) found = 0;
   __syncthreads();
-  // the slices' bins, every GROUPS-th by 256 threads each
-  constexpr int GROUPS = NT / BINS;
   unsigned long long q = 0ull;
   int c = 0;
 #pragma unroll 8
-  for (int i = b / BINS; i < P; i += GROUPS) {
-    const int k = b % BINS - shift[i];
+  for (int i = 0; i < P; ++i) {
+    const int k = b - shift[i];
     const unsigned long long v = s.bins[i * BINS + max(k, 0)];
     if (k >= 0) {
       c += (int)(v >> 48);
       q += v & 0xffffffffffffull;
     }
   }
-  if (!bin) { other_q[b / BINS - 1][b % BINS] = q; other_c[b / BINS - 1][b % BINS] = c; }
-  __syncthreads();
-  if (bin)
-#pragma unroll
-    for (int i = 0; i < GROUPS - 1; ++i) { q += other_q[i][b]; c += other_c[i][b]; }
   // a bin's middle beside the largest; beside an infinite one, or one beyond the lattice, only its equals count
   const bool flat = top == INFINITY || !(fabs((double)top * per) < LATTICE);
-  double m = !bin ? 0.0 : flat ? (b == 0 ? (double)c : 0.0) : (double)q * (1.0 / BIN_ONE) * exp_down((first - b + 0.5 - line) * (1.0 / PER_T));
+  double m = flat ? (b == 0 ? (double)c : 0.0) : (double)q * (1.0 / BIN_ONE) * exp_down((first - b + 0.5 - line) * (1.0 / PER_T));
   const int c_own = c;
-  if (bin) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int cc = __shfl_up(c, o, 64);
-      const double mm = __shfl_up(m, o, 64);
-      if (lane >= o) { c += cc; m += mm; }
-    }
-    if (lane == 63) { wave_c[wave] = c; wave_m[wave] = m; }
-  }
-  __syncthreads();
-  if (bin) {
-    for (int w = 0; w < wave; ++w) { c += wave_c[w]; m += wave_m[w]; }
-    c_in[b] = c;
-    m_in[b] = m;
-  }
+  c = sum_upto<NT>(c, wave_c);
+  m = sum_upto<NT>(m, wave_m);
+  c_in[b] = c;
+  m_in[b] = m;
   __syncthreads();
   const int c_all = c_in[BINS - 1];
-  const double all = m_in[BINS - 1], slack = 1e-11 * all, m_ex = b > 0 && bin ? m_in[b - 1] : 0.0;
+  const double all = m_in[BINS - 1], slack = 1e-11 * all, m_ex = b > 0 ? m_in[b - 1] : 0.0;
   // the bins that each end may lie in: k0, [p0, p1], [m0, m1], [d0, d1]; BINS: nowhere
   const int k = set.m > 1.0 ? 1 : set.k;
   const bool whole = top_k && top_k[r] >= 1 && top_k[r] <= K_COUNT, k_binds = k < c_all;
-  const int k0 = k_binds ? __syncthreads_count(bin && c < k) : BINS;
+  const int k0 = k_binds ? __syncthreads_count(c < k) : BINS;
   const bool k_exact = k_binds && c_in[k0] == k;
   bool p_binds = false, m_binds = false;
   int m0 = BINS, m1 = BINS, from[4] = {0, BINS, BINS, BINS}, to[4] = {min(k0, BINS - 1), -1, -1, -1};       // runs of bins that are wanted
@@ -460,8 +459,8 @@ __global__ __launch_bounds__(NT) void sample_collect_kernel(char* __restrict__ s
     const double mk_hi = k_binds ? m_in[k0] : all, mk_lo = !k_binds || k_exact ? mk_hi : k0 > 0 ? m_in[k0 - 1] : 0.0;
     int p0 = BINS, p1 = BINS;
     if (set.p < 1.0) {
-      p0 = __syncthreads_count(bin && m < set.p * mk_lo - slack);
-      p1 = max(0, __syncthreads_count(bin && m_ex < set.p * mk_hi + slack) - 1);
+      p0 = __syncthreads_count(m < set.p * mk_lo - slack);
+      p1 = max(0, __syncthreads_count(m_ex < set.p * mk_hi + slack) - 1);
     }
     if (set.m > 0.0 && set.m <= 1.0) {
       const double off = fabs(line) * 1e-15 + 1e-6, at = first - line - PER_T * log(set.m);
@@ -476,7 +475,7 @@ __global__ __launch_bounds__(NT) void sample_collect_kernel(char* __restrict__ s
     if (p_binds) { lo = fmin(lo, set.p * mk_lo - slack); hi = fmin(hi, m_in[min(p1, BINS - 1)]); }
     if (m_binds) { lo = fmin(lo, m0 > 0 ? m_in[m0 - 1] : 0.0); hi = fmin(hi, m_in[m1]); }
     lo = fmax(lo, 0.0);
-    const int d0 = __syncthreads_count(bin && m <= set.u * lo - slack), d1 = __syncthreads_count(bin && m_ex <= set.u * hi + slack) - 1;
+    const int d0 = __syncthreads_count(m <= set.u * lo - slack), d1 = __syncthreads_count(m_ex <= set.u * hi + slack) - 1;
     from[0] = d0;
     to[0] = min(d1, end);
     if (p_binds) { from[1] = p0; to[1] = min(p1, end); }
@@ -484,61 +483,55 @@ __global__ __launch_bounds__(NT) void sample_collect_kernel(char* __restrict__ s
     if (k_binds && !k_exact && (k0 <= end || p_binds)) from[3] = to[3] = k0;
   }
   auto wanted = [&](int j) { return (j >= from[0] && j <= to[0]) || (j >= from[1] && j <= to[1]) || (j >= from[2] && j <= to[2]) || (j >= from[3] && j <= to[3]); };
-  const bool flag = bin && wanted(b);
-  int g = 0;
-  if (bin) {
-    const unsigned long long bal = __ballot(flag);
-    g = __popcll(bal & ((1ull << lane) - 1ull));
-    if (lane == 0) wave_s[wave] = __popcll(bal);
-  }
-  // the wanted runs as values: the least float of a run's last bin (of those that this slice has counted: 256 from its own largest on), the least above its first
+  const bool flag = wanted(b);
+  // the wanted runs as values: the least float of a run's last bin the least above its first
   if (b >= NT - 8) {
     const int i = (b & 7) >> 1, above = b & 1, f = i == 0 ? from[0] : i == 1 ? from[1] : i == 2 ? from[2] : from[3], t = i == 0 ? to[0] : i == 1 ? to[1] : i == 2 ? to[2] : to[3];
-    const double floor_of = first - shift[p] - (BINS - 1);
     float v;
     if (flat || !(per > 0.0)) v = above ? NAN : f <= 0 && t >= 0 ? (flat ? top : -3.402823466e38f) : NAN;
-    else v = least_at(above ? first - f + 1.0 : fmax(first - t, floor_of), per);
+    else v = least_at(above ? first - f + 1.0 : first - t, per);
     bounds[i][above] = v;
   }
   __syncthreads();
-  if (p == 0 && bin) {
-    for (int w = 0; w < wave; ++w) g += wave_s[w];
+  if (blockIdx.x == 0) {
+    // (a bin's place among the wanted ones: the runs may touch, so they are counted)
+    const int g = sum_upto<NT>((int)flag, wave_c);
     RowSums& o = *s.sums;
     o.mass[b] = m_ex;
     o.count[b] = c - c_own;
-    o.slot[b] = flag ? (short)g : (short)-1;
-    if (b == 0)
-      o.said = RowSaid{all, c_all, wave_s[0] + wave_s[1] + wave_s[2] + wave_s[3], k_binds ? (k_exact ? 2 : 1) : 0, k0, m0, m1, p_binds, m_binds, whole, 0};
+    o.slot[b] = flag ? (short)(g - 1) : (short)-1;
+    if (b == BINS - 1) o.said = RowSaid{all, c_all, g, k_binds ? (k_exact ? 2 : 1) : 0, k0, m0, m1, p_binds, m_binds, whole, 0};
   }
-  // this slice's: none where none of its bins are wanted
-  const int own = b - shift[p];
-  if (!__syncthreads_or(bin && flag && own >= 0 && s.bins[p * BINS + max(own, 0)] > 0ull)) return;
-  if constexpr (!EARLY) load_slice<NT, NE, VEC>(x, logits + (long)r * ld, base, V);
-  unsigned mask = 0u;
+  unsigned long long* const to_found = s.found + (long)blockIdx.x * cut.cap;
+  for (;;) {
+    unsigned mask = 0u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (from[i] <= to[i]) {
-      const float lo = bounds[i][0], hi = bounds[i][1];
+    for (int i = 0; i < 4; ++i)
+      if (from[i] <= to[i]) {
+        const float lo = bounds[i][0], hi = bounds[i][1];
 #pragma unroll
-      for (int e = 0; e < NE; ++e) mask |= x[e] >= lo && !(x[e] >= hi) ? 1u << e : 0u;
-    }
-  int n = __popc(mask), at = n;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(at, o, 64); if (lane >= o) at += v; }
-  const int sum = __shfl(at, 63, 64);
-  if (sum > 0) {
-    int start = 0;
-    if (lane == 0) start = atomicAdd(&found, sum);
-    at += __shfl(start, 0, 64) - n;
-#pragma unroll
-    for (int e = 0; e < NE; ++e)
-      if (mask >> e & 1) {
-        if (at < SLICE_CAP) s.found[(long)p * SLICE_CAP + at] = ((unsigned long long)key_of(x[e]) << 32) | (unsigned)(0x7fffffff - index_of<NT, NE, VEC>(base, e));
-        ++at;
+        for (int e = 0; e < NE; ++e) mask |= x[e] >= lo && !(x[e] >= hi) ? 1u << e : 0u;
       }
+    if (__ballot(mask != 0u)) {              // (one atomic a wave)
+      const int n = __popc(mask);
+      int at = n, start = 0;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(at, o, 64); if (lane >= o) at += v; }
+      if (lane == 63) start = atomicAdd(&found, at);
+      at += __shfl(start, 63, 64) - n;
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+        if (mask >> e & 1) {
+          if (at < cut.cap) to_found[at] = ((unsigned long long)key_of(x[e]) << 32) | (unsigned)(0x7fffffff - index_of<NT, NE, VEC>(p * NT * NE, e));
+          ++at;
+        }
+    }
+    p += gridDim.x;
+    if (p >= P) break;
+    load_slice<NT, NE, VEC>(x, logits + (long)r * ld, p * NT * NE, V);
   }
   __syncthreads();
-  if (b == 0) s.heads[p].found = found;
+  if (b == 0) s.taken[blockIdx.x] = found;
 }
 
 // Largest first, `n` a power of two of 64 to 2 ST.  Two neighbours a thread: partners at most 64 places apart are in the same wave and change places by
@@ -576,24 +569,9 @@ __device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
   if (on) { v[i0] = a; v[i0 + 1] = b; }
   __syncthreads();
 }
-// sums over the threads in front of each, and with it
-template <typename T> __device__ __forceinline__ T sum_upto(T v, T* room /* ST / 64 */, bool busy = true) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (busy)                                  // (a wave of zeros has no sums to form)
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const T x = __shfl_up(v, o, 64); if (lane >= o) v += x; }
-  __syncthreads();
-  if (lane == 63) room[wave] = v;
-  __syncthreads();
-  T w = lane < wave ? room[lane & (ST / 64 - 1)] : T(0);
-#pragma unroll
-  for (int o = ST / 128; o > 0; o >>= 1) w += __shfl_xor(w, o, 64);
-  return v + __shfl(w, 0, 64);
-}
-
 // a workgroup a row
 template <bool SMALL>
-__global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ tokens, float* __restrict__ probs, char* __restrict__ scratch, int P, int slice,
+__global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ tokens, float* __restrict__ probs, char* __restrict__ scratch, Cut row_cut,
                                                             const float* __restrict__ logits, long ld, int V, const float* __restrict__ uniforms,
                                                             const float* __restrict__ temperature, const int* __restrict__ top_k, const float* __restrict__ top_p,
                                                             const float* __restrict__ min_p) {
@@ -612,7 +590,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* row = logits + (long)r * ld;
   const RowSettings set = row_settings(r, V, temperature, top_k, top_p, min_p, uniforms);
-  const Scratch s = SMALL ? Scratch{} : scratch_of(scratch, r, P, slice);
+  const Scratch s = SMALL ? Scratch{} : scratch_of(scratch, r, row_cut);
   float top = -INFINITY;
   int first_at = 0, had = 0;
   RowSaid said{};
@@ -634,11 +612,11 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     top = of_key((unsigned)(best >> 32));
     first_at = 0x7fffffff - (int)(best & 0xffffffffu);
   } else {
-    const SliceHead h = lane < P ? s.heads[lane] : SliceHead{-INFINITY, 0, 0, 0};
+    const SliceHead h = lane < row_cut.P ? s.heads[lane] : SliceHead{-INFINITY, 0, {0, 0}};
     top = wave_max(h.top);
     const unsigned long long bal = __ballot(h.top == top);
     first_at = __shfl(h.at, __ffsll(bal) - 1, 64);
-    had = h.found;
+    had = lane < row_cut.Q ? s.taken[lane] : 0;
   }
   if (!(top > -INFINITY) || set.greedy) {
     if (tid == 0) {
@@ -655,18 +633,18 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   const int k = set.m > 1.0 ? 1 : set.k;
   int m0 = 0, m1 = BINS - 1, found = 0;
   if constexpr (!SMALL) {
-    if (__ballot(had > slice / 4)) {
+    if (__ballot(had > row_cut.cap)) {
       sample_slow(r, tokens, probs, row, V, set, top, room);
       return;
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(had, o, 64); if (lane >= o) had += x; }
     if (wave == 0) {
-      if (lane < P) from[lane + 1] = had;
+      if (lane < row_cut.Q) from[lane + 1] = had;
       if (lane == 0) from[0] = 0;
     }
     __syncthreads();
-    n = found = from[P];
+    n = found = from[row_cut.Q];
     whole = said.whole;
     if (!whole) {
       p_binds = said.p_binds;
@@ -700,7 +678,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
         const int i = i0 + e * ST;
         if (i < found) {
           while (from[at + 1] <= i) ++at;
-          t[e] = s.found[(long)at * (slice / 4) + i - from[at]];
+          t[e] = s.found[(long)at * row_cut.cap + i - from[at]];
         }
       }
 #pragma unroll
@@ -765,8 +743,8 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     const int b0 = 2 * tid;
     const u64 q0 = raw[b0], q1 = raw[b0 + 1];
     const int c0 = start[b0], c1 = start[b0 + 1];
-    const u64 qs = sum_upto(q0 + q1, wide);
-    const int cs = sum_upto(c0 + c1, narrow);
+    const u64 qs = sum_upto<ST>(q0 + q1, wide);
+    const int cs = sum_upto<ST>(c0 + c1, narrow);
     __syncthreads();
     raw[b0] = qs - q0 - q1;
     raw[b0 + 1] = qs - q1;
@@ -873,7 +851,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       bin[e] = place(v[e0 + e]);
       if (e0 + e == 0 || place(v[e0 + e - 1]) != bin[e]) start[bin[e]] = e0 + e;
     }
-  const u64 sum = sum_upto(q[0] + q[1], wide, 128 * wave < n);
+  const u64 sum = sum_upto<ST>(q[0] + q[1], wide, 128 * wave < n);
   raw[e0] = sum - q[1];
   raw[e0 + 1] = sum;
   __syncthreads();
@@ -933,13 +911,9 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     }
 }
 
-// slices of 32768 values where rows fill the chip by themselves, of 8192 where they do not (one row of 128256: 16 workgroups instead of 4)
-static int slice_values(int rows, int V) { return rows >= 64 ? 32768 : 8192; }
-static int slices_of(int rows, int V) { const int n = slice_values(rows, V); return (V + n - 1) / n; }
-
 extern "C" long umb_sample_requests_bytes(int rows, int V) {
   if (rows < 1 || V < 1 || V > SAMPLE_VMAX) return 0;
-  return V <= SMALL_V ? 16 : rows * row_bytes(slices_of(rows, V), slice_values(rows, V));
+  return V <= SMALL_V ? 16 : rows * row_bytes(cut_of(rows, V));
 }
 
 extern "C" int umb_sample_requests(int* tokens, float* probs, const float* logits, long ld, int rows, int V, const float* uniforms,
@@ -949,28 +923,28 @@ extern "C" int umb_sample_requests(int* tokens, float* probs, const float* logit
       scratch_bytes < umb_sample_requests_bytes(rows, V))
     return UMB_EINVAL;
   if (V <= SMALL_V) {
-    hipLaunchKernelGGL((sample_resolve_kernel<true>), dim3(rows), dim3(ST), 0, st, tokens, probs, (char*)nullptr, 0, 0, logits, ld, V, uniforms, temperature, top_k, top_p,
-                       min_p);
+    hipLaunchKernelGGL((sample_resolve_kernel<true>), dim3(rows), dim3(ST), 0, st, tokens, probs, (char*)nullptr, Cut{}, logits, ld, V, uniforms, temperature, top_k,
+                       top_p, min_p);
     UMB_LAUNCH_CHECK();
     return UMB_OK;
   }
-  const int P = slices_of(rows, V), slice = slice_values(rows, V);
-  const bool vec = (uintptr_t)logits % 16 == 0 && ld % 4 == 0, large = slice == 32768;
-  char* room = static_cast<char*>(scratch);
+  const Cut cut = cut_of(rows, V);
+  const bool vec = (uintptr_t)logits % 16 == 0 && ld % 4 == 0;
   for (int r0 = 0; r0 < rows; r0 += 65535) {                 // (a grid's rows)
     const int n = rows - r0 < 65535 ? rows - r0 : 65535;
-    char* const sc = room + r0 * row_bytes(P, slice);
+    char* const sc = static_cast<char*>(scratch) + r0 * row_bytes(cut);
     const float* const x = logits + r0 * ld;
     auto at = [&](auto* p) { return p ? p + r0 : p; };
-#define SLICES(NT, NE, VEC)                                                                                                                                 \
-  hipLaunchKernelGGL((sample_slices_kernel<NT, NE, VEC>), dim3(P, n), dim3(NT), 0, st, sc, x, ld, V, at(temperature), at(top_k));                                       \
-  hipLaunchKernelGGL((sample_collect_kernel<NT, NE, VEC>), dim3(P, n), dim3(NT), 0, st, sc, x, ld, V, at(uniforms), at(temperature), at(top_k), at(top_p), at(min_p))
-    if (large && vec) { SLICES(1024, 32, true); }
-    else if (large) { SLICES(1024, 32, false); }
-    else if (vec) { SLICES(512, 16, true); }
-    else { SLICES(512, 16, false); }
+#define SLICES(NT, NE, VEC)                                                                                                                         \
+  hipLaunchKernelGGL((sample_slices_kernel<NT, NE, VEC>), dim3(cut.P, n), dim3(NT), 0, st, sc, cut, x, ld, V, at(temperature), at(top_k));           \
+  hipLaunchKernelGGL((sample_collect_kernel<NT * NE / BINS, VEC>), dim3(cut.Q, n), dim3(BINS), 0, st, sc, cut, x, ld, V, at(uniforms), at(temperature), \
+                     at(top_k), at(top_p), at(min_p))
+    if (cut.slice == 8192 && vec) { SLICES(512, 16, true); }
+    else if (cut.slice == 8192) { SLICES(512, 16, false); }
+    else if (vec) { SLICES(512, 32, true); }
+    else { SLICES(512, 32, false); }
 #undef SLICES
-    hipLaunchKernelGGL((sample_resolve_kernel<false>), dim3(n), dim3(ST), 0, st, at(tokens), at(probs), sc, P, slice, x, ld, V, at(uniforms), at(temperature), at(top_k),
+    hipLaunchKernelGGL((sample_resolve_kernel<false>), dim3(n), dim3(ST), 0, st, at(tokens), at(probs), sc, cut, x, ld, V, at(uniforms), at(temperature), at(top_k),
                        at(top_p), at(min_p));
     UMB_LAUNCH_CHECK();
   }
