@@ -378,27 +378,54 @@ __global__ __launch_bounds__(NT) void sample_slices_kernel(char* __restrict__ sc
   for (int i = threadIdx.x; i < BINS; i += NT) s.bins[p * BINS + i] = bins[i];
 }
 
-// sums over the threads in front of each, and with it, of a workgroup of NT; `busy` false: this wave's are zeros
-template <int NT, typename T> __device__ __forceinline__ T sum_upto(T v, T* room /* NT / 64 */, bool busy = true) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (busy)
+// another lane's value by the vector unit alone; lanes that have none get 0
+template <int CTRL, int ROWS, typename T> __device__ __forceinline__ T lanes(T v) {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 8);
+  int w[sizeof(T) / 4];
+  __builtin_memcpy(w, &v, sizeof v);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const T x = __shfl_up(v, o, 64); if (lane >= o) v += x; }
+  for (int i = 0; i < (int)(sizeof(T) / 4); ++i) w[i] = __builtin_amdgcn_update_dpp(0, w[i], CTRL, ROWS, 0xf, false);
+  T r;
+  __builtin_memcpy(&r, w, sizeof r);
+  return r;
+}
+// sums over a wave's lanes in front of each, and with it: within rows of 16, then the rows in front
+template <typename T> __device__ __forceinline__ T wave_upto(T v) {
+  v += lanes<0x111, 0xf>(v);
+  v += lanes<0x112, 0xf>(v);
+  v += lanes<0x114, 0xf>(v);
+  v += lanes<0x118, 0xf>(v);
+  v += lanes<0x142, 0xa>(v);
+  v += lanes<0x143, 0xc>(v);
+  return v;
+}
+// the same over a workgroup of NT
+template <int NT, typename T> __device__ __forceinline__ T sum_upto(T v, T* room /* NT / 64 */) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  static_assert(NT <= 1024);
+  v = wave_upto(v);
   __syncthreads();
   if (lane == 63) room[wave] = v;
   __syncthreads();
-  T w = lane < wave ? room[lane & (NT / 64 - 1)] : T(0);
-#pragma unroll
-  for (int o = NT / 128; o > 0; o >>= 1) w += __shfl_xor(w, o, 64);
-  return v + __shfl(w, 0, 64);
+  T w = lane < NT / 64 ? room[lane] : T(0);
+  w += lanes<0x111, 0xf>(w);
+  w += lanes<0x112, 0xf>(w);
+  w += lanes<0x114, 0xf>(w);
+  w += lanes<0x118, 0xf>(w);
+  const T before = __shfl(w, wave > 0 ? wave - 1 : 0, 64);
+  return wave > 0 ? v + before : v;
 }
-
-// how many of `n` bins in a row, NB a thread, have what holds for the first of them and not for the rest
-template <int NB> __device__ __forceinline__ int bins_with(const bool (&holds)[NB]) {
-  int n = 0;
+// how many threads of NT hold a, and how many b; `room` [NT / 64] is this call's alone
+struct Two { int a, b; };
+template <int NT> __device__ __forceinline__ Two how_many(bool a, bool b, int* room) {
+  const int lane = threadIdx.x & 63;
+  const int n = __popcll(__ballot(a)) | (__popcll(__ballot(b)) << 16);
+  if (lane == 0) room[threadIdx.x >> 6] = n;
+  __syncthreads();
+  int w = 0;
 #pragma unroll
-  for (int e = 0; e < NB; ++e) n += __syncthreads_count(holds[e]);
-  return n;
+  for (int i = 0; i < NT / 64; ++i) w += room[i];
+  return Two{w & 0xffff, w >> 16};
 }
 
 // grid (Q, rows); a thread a bin
@@ -408,7 +435,7 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
                                                               const float* __restrict__ top_p, const float* __restrict__ min_p) {
   constexpr int NT = BINS;
   __shared__ double m_in[BINS], wave_m[NT / 64];
-  __shared__ int shift[P_MAX], c_in[BINS], wave_c[NT / 64], found;
+  __shared__ int shift[P_MAX], c_in[BINS], wave_c[NT / 64], rooms[3][NT / 64], found;
   __shared__ float bounds[4][2];
   const int r = blockIdx.y, P = cut.P, b = threadIdx.x, lane = b & 63;
   int p = blockIdx.x;                        // chunk
@@ -451,7 +478,7 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
   // the bins that each end may lie in: k0, [p0, p1], [m0, m1], [d0, d1]; BINS: nowhere
   const int k = set.m > 1.0 ? 1 : set.k;
   const bool whole = top_k && top_k[r] >= 1 && top_k[r] <= K_COUNT, k_binds = k < c_all;
-  const int k0 = k_binds ? __syncthreads_count(c < k) : BINS;
+  const int k0 = k_binds ? how_many<NT>(c < k, false, rooms[0]).a : BINS;
   const bool k_exact = k_binds && c_in[k0] == k;
   bool p_binds = false, m_binds = false;
   int m0 = BINS, m1 = BINS, from[4] = {0, BINS, BINS, BINS}, to[4] = {min(k0, BINS - 1), -1, -1, -1};       // runs of bins that are wanted
@@ -459,8 +486,9 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
     const double mk_hi = k_binds ? m_in[k0] : all, mk_lo = !k_binds || k_exact ? mk_hi : k0 > 0 ? m_in[k0 - 1] : 0.0;
     int p0 = BINS, p1 = BINS;
     if (set.p < 1.0) {
-      p0 = __syncthreads_count(m < set.p * mk_lo - slack);
-      p1 = max(0, __syncthreads_count(m_ex < set.p * mk_hi + slack) - 1);
+      const Two n = how_many<NT>(m < set.p * mk_lo - slack, m_ex < set.p * mk_hi + slack, rooms[1]);
+      p0 = n.a;
+      p1 = max(0, n.b - 1);
     }
     if (set.m > 0.0 && set.m <= 1.0) {
       const double off = fabs(line) * 1e-15 + 1e-6, at = first - line - PER_T * log(set.m);
@@ -475,7 +503,8 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
     if (p_binds) { lo = fmin(lo, set.p * mk_lo - slack); hi = fmin(hi, m_in[min(p1, BINS - 1)]); }
     if (m_binds) { lo = fmin(lo, m0 > 0 ? m_in[m0 - 1] : 0.0); hi = fmin(hi, m_in[m1]); }
     lo = fmax(lo, 0.0);
-    const int d0 = __syncthreads_count(m <= set.u * lo - slack), d1 = __syncthreads_count(m_ex <= set.u * hi + slack) - 1;
+    const Two d = how_many<NT>(m <= set.u * lo - slack, m_ex <= set.u * hi + slack, rooms[2]);
+    const int d0 = d.a, d1 = d.b - 1;
     from[0] = d0;
     to[0] = min(d1, end);
     if (p_binds) { from[1] = p0; to[1] = min(p1, end); }
@@ -534,41 +563,80 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
   if (b == 0) s.taken[blockIdx.x] = found;
 }
 
-// Largest first, `n` a power of two of 64 to 2 ST.  Two neighbours a thread: partners at most 64 places apart are in the same wave and change places by
-// shuffles, others through LDS.
-__device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
-  typedef unsigned long long u64;
-  const int i0 = 2 * threadIdx.x;
-  const bool on = i0 < n, busy = (i0 & ~127) < n;            // (a wave that has none of them leaves the others LDS's time)
-  __syncthreads();
-  u64 a = on ? v[i0] : 0ull, b = on ? v[i0 + 1] : 0ull;
-  for (int k = 2; k <= n; k <<= 1) {
-    const bool down = (i0 & k) == 0;
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      if (j == 1) {
-        if ((a < b) == down) { const u64 t = a; a = b; b = t; }
-      } else if (busy || j > 64) {
-        u64 c, d;
-        if (j <= 64) {
-          c = __shfl_xor(a, j >> 1, 64);
-          d = __shfl_xor(b, j >> 1, 64);
-        } else {
-          __syncthreads();
-          if (on) { v[i0] = a; v[i0 + 1] = b; }
-          __syncthreads();
-          c = on ? v[i0 ^ j] : 0ull;
-          d = on ? v[(i0 ^ j) + 1] : 0ull;
-        }
-        const bool large = ((i0 & j) == 0) == down;        // of a pair the one in front takes the larger one, where it runs down
-        a = (a < c) == large ? c : a;
-        b = (b < d) == large ? d : b;
-      }
-    }
+// lane ^ X's value by the vector unit alone
+template <int X> __device__ __forceinline__ unsigned lane_xor(unsigned v) {
+  static_assert(X == 1 || X == 2 || X == 3 || X == 4 || X == 7 || X == 8 || X == 15 || X == 16 || X == 31 || X == 63);
+  if constexpr (X == 4) return lane_xor<3>(lane_xor<7>(v));
+  else if constexpr (X == 31) return lane_xor<16>(lane_xor<15>(v));
+  else if constexpr (X == 63) {
+    const unsigned w = lane_xor<31>(v);
+    const auto a = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return threadIdx.x & 32 ? a[0] : a[1];
+  } else if constexpr (X == 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? a[0] : a[1];
+  } else {
+    constexpr int ctrl = X == 1 ? 0xb1 : X == 2 ? 0x4e : X == 3 ? 0x1b : X == 7 ? 0x141 : X == 15 ? 0x140 : 0x128;
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false);
   }
-  __syncthreads();
-  if (on) { v[i0] = a; v[i0 + 1] = b; }
-  __syncthreads();
 }
+// of lanes whose numbers differ by X the one in front takes the larger value
+template <int X> __device__ __forceinline__ void order(unsigned long long& v) {
+  constexpr int top = X >= 32 ? 32 : X >= 16 ? 16 : X >= 8 ? 8 : X >= 4 ? 4 : X >= 2 ? 2 : 1;
+  const unsigned long long o = lane_xor<X>((unsigned)v) | ((unsigned long long)lane_xor<X>((unsigned)(v >> 32)) << 32);
+  v = (v < o) == ((threadIdx.x & top) == 0) ? o : v;
+}
+__device__ __forceinline__ void sort_wave(unsigned long long& v) {
+  order<1>(v);
+  order<3>(v), order<1>(v);
+  order<7>(v), order<2>(v), order<1>(v);
+  order<15>(v), order<4>(v), order<2>(v), order<1>(v);
+  order<31>(v), order<8>(v), order<4>(v), order<2>(v), order<1>(v);
+  order<63>(v), order<16>(v), order<8>(v), order<4>(v), order<2>(v), order<1>(v);
+}
+// Largest first, `n` a power of two of 64 to 2 ST, values that differ (or are 0).  Runs of 64 by the lanes of a wave, then pairs of runs: a value's place is its own plus
+// how many of the other run are larger.  w: room for as many.
+__device__ __forceinline__ void sort_down(unsigned long long* v, unsigned long long* w, int n) {
+  typedef unsigned long long u64;
+  const int lane = threadIdx.x & 63, i0 = (threadIdx.x >> 6) * 128 + lane;
+  const bool on[2] = {i0 < n, i0 + 64 < n};
+  __syncthreads();
+  u64 a[2] = {on[0] ? v[i0] : 0ull, on[1] ? v[i0 + 64] : 0ull};
+  int at[2] = {i0, i0 + 64};
+  if (on[0]) {                               // (a wave's are there or not together)
+    sort_wave(a[0]);
+    sort_wave(a[1]);
+  }
+  int turns = 0;
+  while (64 << turns < n) ++turns;
+  u64 *to = turns & 1 ? w : v, *other = turns & 1 ? v : w;
+  for (int run = 64;; run <<= 1) {
+    __syncthreads();                         // (the first: all have been read; then: the buffer before last has)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) if (on[e]) to[at[e]] = a[e];
+    __syncthreads();
+    if (run >= n) break;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (on[e]) {
+        const int base = (at[e] & ~(run - 1)) ^ run;         // the other run
+        const bool second = (at[e] & run) != 0;              // of equals (zeros) the first run's stand in front
+        int lo = 0;
+        for (int step = run; step > 0; step >>= 1) {
+          const int m = lo + step;
+          if (m <= run) {
+            const u64 x = to[base + m - 1];
+            if (x > a[e] || (second && x == a[e])) lo = m;
+          }
+        }
+        at[e] = (at[e] & ~(2 * run - 1)) + (at[e] & (run - 1)) + lo;
+      }
+    u64* const t = to;
+    to = other;
+    other = t;
+  }
+}
+
 // a workgroup a row
 template <bool SMALL>
 __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ tokens, float* __restrict__ probs, char* __restrict__ scratch, Cut row_cut,
@@ -580,7 +648,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   __shared__ double front_m[CAP];                                  // mass and count in front of each bin
   __shared__ int front_c[CAP], start[CAP];                         // where a bin's tokens start in v
   __shared__ u64 wide[ST / 64];
-  __shared__ int narrow[ST / 64];
+  __shared__ int narrow[ST / 64], rooms[6][ST / 64];
   __shared__ short slot[BINS], bin_of[BINS];
   __shared__ unsigned char want[CAP];
   __shared__ SlowRoom room;
@@ -778,8 +846,11 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       mass = masses;
     }
     const double slack = slack_of * mass;
-    auto before = [&](bool a, bool b) { const bool h[2] = {is[0] && a, is[1] && b}; return bins_with(h); };
-    const int k0 = how_k == 1 ? before(c_in[0] < k, c_in[1] < k) : used;
+    auto before = [&](bool a0, bool a1, bool b0, bool b1, int call) -> Two {       // bins, of both a thread's
+      const Two x = how_many<ST>(is[0] && a0, is[0] && b0, rooms[2 * call]), y = how_many<ST>(is[1] && a1, is[1] && b1, rooms[2 * call + 1]);
+      return Two{x.a + y.a, x.b + y.b};
+    };
+    const int k0 = how_k == 1 ? before(c_in[0] < k, c_in[1] < k, false, false, 0).a : used;
     double lo = mass, hi = mass;
     if (k0 < used) {
       __syncthreads();
@@ -797,9 +868,10 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     }
     int p0 = used, p1 = -1;
     if (p_binds) {
-      p0 = before(in[0] < set.p * lo - slack, in[1] < set.p * lo - slack);
-      p1 = before(ex[0] < set.p * hi + slack, ex[1] < set.p * hi + slack) - 1;
-      p1 = max(p1, 0);
+      const double l = set.p * lo - slack, h = set.p * hi + slack;
+      const Two n = before(in[0] < l, in[1] < l, ex[0] < h, ex[1] < h, 1);
+      p0 = n.a;
+      p1 = max(n.b - 1, 0);
       if (p0 < used) {
         lo = fmin(lo, set.p * lo - slack);
         __syncthreads();
@@ -812,7 +884,8 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     if (m_binds) { lo = fmin(lo, end_m - slack); hi = fmin(hi, end_m + slack); }
     lo = fmax(lo, 0.0);
     const double ulo = set.u * lo - slack, uhi = set.u * hi + slack;
-    const int d0 = before(in[0] <= ulo, in[1] <= ulo), d1 = before(ex[0] <= uhi, ex[1] <= uhi) - 1;
+    const Two d = before(in[0] <= ulo, in[1] <= ulo, ex[0] <= uhi, ex[1] <= uhi, 2);
+    const int d0 = d.a, d1 = d.b - 1;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int b = b0 + e;
@@ -837,7 +910,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   int size = 64;
   while (size < n) size <<= 1;
   for (int i = n + tid; i < size; i += ST) v[i] = 0ull;
-  sort_down(v, size);
+  sort_down(v, raw, size);
   // mass up to and with each token, and its rank
   const int e0 = 2 * tid;
   u64 q[2] = {0ull, 0ull};
@@ -851,7 +924,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       bin[e] = place(v[e0 + e]);
       if (e0 + e == 0 || place(v[e0 + e - 1]) != bin[e]) start[bin[e]] = e0 + e;
     }
-  const u64 sum = sum_upto<ST>(q[0] + q[1], wide, 128 * wave < n);
+  const u64 sum = sum_upto<ST>(q[0] + q[1], wide);
   raw[e0] = sum - q[1];
   raw[e0 + 1] = sum;
   __syncthreads();
