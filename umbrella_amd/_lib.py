@@ -425,18 +425,18 @@ def load_seq() -> C.CDLL:
     return lib
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # the address alone, without torch.cuda.current_stream()'s 2 us
+
+
+def _stream_of(index: int) -> int:
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def seq_call(name: str, *args):
     """call an entry point of libumbrella_seq.so on the current stream (tensors -> pointers, structs by reference)"""
-    lib = load_seq()
-    conv = []
-    for a in args:
-        if isinstance(a, torch.Tensor) or a is None:
-            conv.append(ptr(a))
-        elif isinstance(a, C.Structure):
-            conv.append(C.byref(a))
-        else:
-            conv.append(a)
-    rc = getattr(lib, name)(*conv, stream_ptr())
+    lib = _seq_lib or load_seq()
+    conv = [a.data_ptr() if isinstance(a, torch.Tensor) else C.byref(a) if isinstance(a, C.Structure) else a for a in args]
+    rc = getattr(lib, name)(*conv, _stream_of(torch.cuda.current_device()))
     if rc != 0:
         raise UmbError(f"libumbrella_seq {name} failed with code {rc}")
 

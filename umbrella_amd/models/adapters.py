@@ -34,28 +34,20 @@ def add_adapters(base, x, a, b, adapter, scale=None, rank=None, out=None):
     base, out: fp32 ``[T, N]`` (out may be base; None: a new tensor); x ``[T, K]``, a ``[S, R, K]``, b ``[S, N, R]`` of one type (bf16, fp16, fp32);
     adapter int32 ``[T]``; scale fp32 ``[S]``; rank int32 ``[S]``: how many of an adapter's R rows count (None: all).  All contiguous, on one GPU.
     """
-    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3 or base.dim() != 2:
-        raise ValueError(f"base [T, N], x [T, K], a [S, R, K] and b [S, N, R] are wanted, got {[tuple(t.shape) for t in (base, x, a, b)]}")
+    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        raise ValueError(f"x [T, K], a [S, R, K] and b [S, N, R] are wanted, got {[tuple(t.shape) for t in (x, a, b)]}")
     (T, K), (S, R, _), N, dev, dt = x.shape, a.shape, b.shape[1], x.device, x.dtype
     code = _lib.seq_dtype_code(dt)
     if dev.type != "cuda":
         raise ValueError(f"tensors on a GPU are wanted, got {dev}")
-    if a.shape[2] != K or b.shape[0] != S or b.shape[2] != R or base.shape != (T, N) or a.dtype != dt or b.dtype != dt or base.dtype != torch.float32:
-        raise ValueError(f"base fp32 [T, N], x [T, K], a [S, R, K] and b [S, N, R] of one type are wanted, got "
-                         f"{[(tuple(t.shape), t.dtype) for t in (base, x, a, b)]}")
     if S < 1 or not 1 <= R <= MAX_RANK or K < 1 or N < 1:
         raise ValueError(f"at least one adapter of a rank of 1 to {MAX_RANK} is wanted, got a of {tuple(a.shape)}")
-    if adapter.shape != (T,) or adapter.dtype != torch.int32:
-        raise ValueError(f"adapter: an int32 number per row is wanted, got {adapter.dtype} {tuple(adapter.shape)}")
-    if (scale is not None and (scale.shape != (S,) or scale.dtype != torch.float32)) or (rank is not None and (rank.shape != (S,) or rank.dtype != torch.int32)):
-        raise ValueError("scale: fp32, rank: int32, one value per adapter")
     if out is None:
-        out = torch.empty_like(base, memory_format=torch.contiguous_format)
-    elif out.shape != base.shape or out.dtype != torch.float32:
-        raise ValueError(f"out: fp32 {tuple(base.shape)} is wanted, got {out.dtype} {tuple(out.shape)}")
-    for t in (base, out, x, a, b, adapter, scale, rank):
-        if t is not None and (t.device != dev or not t.is_contiguous()):
-            raise ValueError("contiguous tensors on one device are wanted")
+        out = torch.empty((T, N), dtype=torch.float32, device=dev)
+    for what, t, shape, kind in (("a", a, (S, R, K), dt), ("b", b, (S, N, R), dt), ("base", base, (T, N), torch.float32), ("out", out, (T, N), torch.float32),
+                                 ("adapter", adapter, (T,), torch.int32), ("scale", scale, (S,), torch.float32), ("rank", rank, (S,), torch.int32), ("x", x, (T, K), dt)):
+        if t is not None and (t.shape != shape or t.dtype != kind or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"{what}: a contiguous {kind} tensor {shape} on {dev} is wanted, got {t.dtype} {tuple(t.shape)} of strides {t.stride()} on {t.device}")
     if T:
         n = _lib.load_seq().umb_seq_adapters_floats(T, K, R)
         scratch = torch.empty(n, dtype=torch.float32, device=dev)
