@@ -669,6 +669,17 @@ int umb_lat_attend_tiled_ok(int H, int kv_rank, int rot_dim, int dtype);
 
 int umb_seq_forward(const UmbSeqModel* m, const UmbSeqWork* ws, const UmbSeqStep* s, umb_stream_t stream);
 
+/* The same step with low-rank adapters (umb_seq_adapters) beside the mixers' input and output products: proj and out are host arrays of a row per layer of the
+ * model (a null: none there); adapter int32 [T] on the device, one of S or none per row.  Seams and products run apart, and an adapted output product sums whole. */
+typedef struct UmbSeqAdapter { const void* a; const void* b; const float* scale; const int32_t* rank; int32_t R, pad_; } UmbSeqAdapter;
+typedef struct UmbSeqAdapters {
+  const UmbSeqAdapter* proj; const UmbSeqAdapter* out;
+  const int32_t* adapter;
+  float* scratch; int64_t scratch_floats;
+  int32_t S, pad_;
+} UmbSeqAdapters;
+int umb_seq_forward_adapters(const UmbSeqModel* m, const UmbSeqWork* ws, const UmbSeqStep* s, const UmbSeqAdapters* adapters, umb_stream_t stream);
+
 /* ------------------------------------------------------------------ steps of many requests at once */
 
 /* The next token of every row of logits (fp32, rows ld apart), each with its own settings: fp32 temperature [rows], int32 top_k, fp32 top_p and min_p

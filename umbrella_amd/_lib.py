@@ -288,6 +288,15 @@ class UmbSeqStep(C.Structure):
                 ("trace", C.c_void_p)]
 
 
+class UmbSeqAdapter(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("rank", C.c_void_p), ("R", C.c_int32), ("pad_", C.c_int32)]
+
+
+class UmbSeqAdapters(C.Structure):
+    _fields_ = [("proj", C.POINTER(UmbSeqAdapter)), ("out", C.POINTER(UmbSeqAdapter)), ("adapter", C.c_void_p), ("scratch", C.c_void_p),
+                ("scratch_floats", C.c_int64), ("S", C.c_int32), ("pad_", C.c_int32)]
+
+
 class UmbSeqFront(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("kind", "W", "groups", "V", "parts", "parts2")] + \
         [(n, C.c_void_p) for n in ("x", "y", "y2", "w_post", "w_next", "w1", "w2", "embed", "tokens", "mix", "out", "in_")] + \
@@ -389,6 +398,7 @@ SEQ_SIGNATURES = {
     "umb_moe_route_softmax": [_P, _P, _P, _P, _I, _I, _I],
     "umb_moe_combine_weighted": [_P, _P, _P, _P, _I, _I, _I, _I],
     "umb_seq_forward": [C.POINTER(UmbSeqModel), C.POINTER(UmbSeqWork), C.POINTER(UmbSeqStep)],
+    "umb_seq_forward_adapters": [C.POINTER(UmbSeqModel), C.POINTER(UmbSeqWork), C.POINTER(UmbSeqStep), C.POINTER(UmbSeqAdapters)],
     "umb_argmax_rows": [_P, _P, _I, _I],
     "umb_sample_rows": [_P, _P, _I, _I, _P, _P, _F, _F, _I, _F, _P, _I, _P, _P],
     "umb_sample_requests_bytes": [_I, _I],

@@ -187,7 +187,10 @@ class PagedSeqCache:
       pooled entries (a ``kv_layers`` entry ``(G, D, 0, E)``);
     * element-wise recurrences use the same state arrays with ``(1, 1, channels)``;
     * nothing is cleared when a slot or a page is handed out again: a sequence that starts at position 0 ignores what its
-      slot holds, and no kernel reads a cache position its own sequence has not written.
+      slot holds, and no kernel reads a cache position its own sequence has not written;
+    * ``fork`` makes sequences that go on from where another one is: they share its full pages, which nobody writes any more (a pooled
+      block lives in the page of its last position), and have copies of the page it has begun and of its slot; a page is free again
+      when the last sequence that holds it is closed.  ``compact`` moves what is held to the front of every store.
 
     Free pages and slots are LIFO stacks, so whatever was given back last is used first.
     """
@@ -219,12 +222,14 @@ class PagedSeqCache:
                      for _ in range(conv_states)] if conv_taps > 0 else []
         self.mixer_conv = [torch.zeros(max_seqs, max(taps - 1, 1), ch, dtype=torch.float32, device=device)
                            for (taps, ch) in mixer_convs]
+        self._pool_rows = None
         self.clear()
 
     def clear(self):
         self.free_pages = list(range(self.n_pages - 1, -1, -1))
         self.free_slots = list(range(self.max_seqs - 1, -1, -1))
         self.seqs = {}                                   # id -> {"slot", "len", "pages"}
+        self.refs = [0] * self.n_pages                   # sequences that hold each page
 
     # ---- bookkeeping (host)
     def open(self, seq_id) -> int:
@@ -238,8 +243,72 @@ class PagedSeqCache:
 
     def close(self, seq_id):
         s = self.seqs.pop(seq_id)
-        self.free_pages.extend(reversed(s["pages"]))
+        for p in reversed(s["pages"]):
+            self.refs[p] -= 1
+            if self.refs[p] == 0:
+                self.free_pages.append(p)
         self.free_slots.append(s["slot"])
+
+    # ---- pages copied (csrc/seq_pages.hip)
+    def _pools(self):
+        """(the stores that pages number, those that slots number) as copy_pages takes them"""
+        if self._pool_rows is None:
+            of_pages = [(t, 1) for c in self.kv for t in (c["k"], c["v"])] + [(t[:, None], 1) for t in self.latent]
+            of_pages += [(t, c["pool"]) for c in self.kv if c["kp"] is not None for t in (c["kp"], c["vp"])]
+            rows = [[t.data_ptr(), t[0].numel() * t.element_size(), t.shape[1], t.shape[2], t.shape[3] * t.element_size(), per] for t, per in of_pages]
+            of_slots = [[t.data_ptr(), t[0].numel() * 4, 1, 1, t[0].numel() * 4, 0] for t in (*self.state, *self.conv, *self.mixer_conv)]
+            of_slots.append([self.pages_dev.data_ptr(), self.max_pages * 4, 1, self.max_pages, 4, self.page])
+            self._pool_rows = tuple(torch.tensor(r, dtype=torch.int64).reshape(-1, 6) for r in (rows, of_slots))
+        return self._pool_rows
+
+    def fork(self, seq_id, children) -> list:
+        """Opens the sequences `children` as copies of an open one, as long as it is; each goes its own way from there.  Returns their slots.
+        What is refused (KeyError: a name in use; RuntimeError: too few slots or pages) changes nothing."""
+        s, children = self.seqs[seq_id], list(children)
+        for c in children:
+            if c in self.seqs or children.count(c) > 1:
+                raise KeyError(f"sequence {c!r} is already open")
+        n, (full, rest) = len(children), divmod(s["len"], self.page)
+        if n > len(self.free_slots):
+            raise RuntimeError(f"no free sequence slot for {n} more ({self.max_seqs - len(self.free_slots)} of {self.max_seqs} in use)")
+        if rest and n > len(self.free_pages):
+            raise RuntimeError(f"paged cache exhausted: {n} pages wanted, {len(self.free_pages)} free ({self.n_pages} pages of {self.page} tokens)")
+        slots, pages = self.free_slots[::-1][:n], self.free_pages[::-1][:n] if rest else []
+        if s["len"] > 0 and n > 0:
+            begun = [(s["pages"][full], p, rest) for p in pages]
+            moves = send(torch.tensor(begun + [(s["slot"], slot, s["len"]) for slot in slots], dtype=torch.int32), self.device)
+            of_pages, of_slots = self._pools()
+            if begun:
+                copy_pages(of_pages, moves[:len(begun)], self.n_pages)
+            copy_pages(of_slots, moves[len(begun):], self.max_seqs)
+            self.write_pages([(slot * self.max_pages + full, p) for slot, p in zip(slots, pages)])
+        for i, c in enumerate(children):
+            self.free_slots.pop()
+            own = [self.free_pages.pop()] if rest else []
+            self.seqs[c] = dict(s, slot=slots[i], pages=s["pages"][:full] + own)
+            for p in self.seqs[c]["pages"]:
+                self.refs[p] += 1
+        return slots
+
+    def compact(self) -> int:
+        """Moves the pages that are held to the front of every store and returns how many they are: what the sequences hold stands in
+        [:n] of each, in one piece, and the pages behind are free."""
+        held = [p for p in range(self.n_pages) if self.refs[p] > 0]
+        n = len(held)
+        into = (p for p in range(n) if self.refs[p] == 0)
+        where = list(range(self.n_pages))
+        moves = [(p, next(into), self.page) for p in held if p >= n]
+        for src, dst, _ in moves:
+            where[src] = dst
+        if moves:
+            both = send(torch.tensor([v for m in moves for v in m] + where, dtype=torch.int32), self.device)
+            copy_pages(self._pools()[0], both[:3 * len(moves)].view(-1, 3), self.n_pages, table=self.pages_dev, where=both[3 * len(moves):])
+            for src, dst, _ in moves:
+                self.refs[dst], self.refs[src] = self.refs[src], 0
+            for s in self.seqs.values():
+                s["pages"] = [where[p] for p in s["pages"]]
+        self.free_pages = list(range(self.n_pages - 1, n - 1, -1))
+        return n
 
     def length(self, seq_id) -> int:
         return self.seqs[seq_id]["len"]
@@ -268,6 +337,8 @@ class PagedSeqCache:
         if need > 0:
             have = len(s["pages"])
             new = [self.free_pages.pop() for _ in range(need)]
+            for p in new:
+                self.refs[p] = 1
             s["pages"].extend(new)
             at = s["slot"] * self.max_pages + have
             added = [(at + i, page) for i, page in enumerate(new)]

@@ -43,6 +43,13 @@ static int lin_y(const UmbSeqLinear& l, float* y, const UmbSeqWork* ws, const vo
   return n > 1 ? umb_seq_linear_parts(y, x, l.w, l.bias, T, l.N, l.K, n, dtype, st) : lin(l, y, x, T, 0, dtype, st);
 }
 
+// a layer's adapter beside its product l: y += scale B A x for the rows that have one
+static int adapt(const UmbSeqAdapters* ad, const UmbSeqAdapter* of, const UmbSeqLinear& l, float* y, const void* x, int T, int dtype, hipStream_t st) {
+  if (!of || !of->a) return UMB_OK;
+  return umb_seq_adapters(y, y, x, of->a, of->b, ad->adapter, of->scale, of->rank, T, l.N, l.K, ad->S, of->R, ad->scratch, ad->scratch_floats, dtype, st);
+}
+static const UmbSeqAdapter* adapter_of(const UmbSeqAdapters* ad, const UmbSeqAdapter* UmbSeqAdapters::*which, int l) { return ad && ad->*which ? ad->*which + l : nullptr; }
+
 static const void* first_norm_of(const UmbSeqModel* m, int l) { return l < m->L ? m->layers[l].norm1 : nullptr; }
 
 // What a sublayer reads.  With a pre-norm the seam kernel has already left norm(x) * w in ws->h.  Without one the sublayer
@@ -496,7 +503,7 @@ static int head_product(const UmbSeqModel* m, const UmbSeqWork* ws, const UmbSeq
 
 // Layers whose sublayers both read the same residual: x <- x + (mixer(norm1 x) + ff(norm2 x)); one seam launch per layer adds
 // both outputs (and, in front of a span that runs again, the embedding row) and norms for the next layer.
-static int forward_parallel_blocks(const UmbSeqModel* m, const UmbSeqWork* ws, const UmbSeqStep* s, hipStream_t st) {
+static int forward_parallel_blocks(const UmbSeqModel* m, const UmbSeqWork* ws, const UmbSeqStep* s, const UmbSeqAdapters* ad, hipStream_t st) {
   const int T = s->T, W = m->W, dt = m->dtype;
   if (!ws->h2 || !ws->y2 || !m->layers[0].norm1 || m->layers[0].add_embed) return UMB_EINVAL;
   const UmbSeqLayer& l0 = m->layers[0];
@@ -507,8 +514,10 @@ static int forward_parallel_blocks(const UmbSeqModel* m, const UmbSeqWork* ws, c
     const UmbSeqLayer* nl = l + 1 < m->L ? &m->layers[l + 1] : nullptr;
     if (!ly.norm1 || (ly.has_mlp && !ly.norm2)) return UMB_EINVAL;
     SEQ_TRY(lin(ly.proj, ws->proj, ws->h, T, 0, dt, st));
+    SEQ_TRY(adapt(ad, adapter_of(ad, &UmbSeqAdapters::proj, l), ly.proj, ws->proj, ws->h, T, dt, st));
     SEQ_TRY(run_mixer(m, ly, ws, s, st));
     SEQ_TRY(lin(ly.out, ws->y, ws->mix, T, 0, dt, st));
+    SEQ_TRY(adapt(ad, adapter_of(ad, &UmbSeqAdapters::out, l), ly.out, ws->y, ws->mix, T, dt, st));
     if (ly.has_mlp) SEQ_TRY(feed_forward(m, ly, ws, s, ws->h2, ws->y2, nullptr, st));
     const float* y2 = ly.has_mlp ? ws->y2 : nullptr;
     const void* w1 = nl ? nl->norm1 : nullptr;
@@ -575,11 +584,11 @@ static int front_product(const UmbSeqModel* m, UmbSeqWork* ws, const UmbSeqStep*
   return UMB_OK;
 }
 
-extern "C" int umb_seq_forward(const UmbSeqModel* m, const UmbSeqWork* given, const UmbSeqStep* s, hipStream_t st) {
+static int forward(const UmbSeqModel* m, const UmbSeqWork* given, const UmbSeqStep* s, const UmbSeqAdapters* ad, hipStream_t st) {
   if (!m || !given || !s || m->L < 1 || !m->layers || s->T < 1 || s->T > given->Tmax || s->B < 1 || s->R < 0 || s->R > given->Rmax ||
       (s->R > 0 && !m->final_norm))
     return UMB_EINVAL;
-  if (m->block == UMB_BLOCK_PARALLEL) return forward_parallel_blocks(m, given, s, st);
+  if (m->block == UMB_BLOCK_PARALLEL) return forward_parallel_blocks(m, given, s, ad, st);
   const int T = s->T, W = m->W, dt = m->dtype, groups = m->groups;
   const float eps = m->eps;
   const bool hyper = m->streams >= 1;          // several residual streams: norms in front only, stream seams
@@ -588,7 +597,8 @@ extern "C" int umb_seq_forward(const UmbSeqModel* m, const UmbSeqWork* given, co
   UmbSeqWork* const ws = &work;
   Pending pend;
   // (rows that the products can leave; a workspace without them goes to the seams, which take any alignment and refuse what is not there)
-  if (S <= 1 && !s->trace && T <= given->Tmax / 2 && given->x && given->h && (uintptr_t)given->x % 16 == 0) pend.spare = given->x + (size_t)T * W;
+  // (and an adapter reads the normed rows, which a product that forms them does not leave)
+  if (!ad && S <= 1 && !s->trace && T <= given->Tmax / 2 && given->x && given->h && (uintptr_t)given->x % 16 == 0) pend.spare = given->x + (size_t)T * W;
   // Every row's logits are wanted, in order (single tokens, scored texts): the last seam norms them for the head, which a launch of its own did in 5 us and
   // more.  (Of several streams the head reads the sum: not a seam's output.)
   const bool whole = s->R == T && !s->logit_rows && (!hyper || S == 1);
@@ -654,8 +664,12 @@ extern "C" int umb_seq_forward(const UmbSeqModel* m, const UmbSeqWork* given, co
     if (!hyper) SEQ_TRY(sublayer_input(m, ws, s, ly.norm1, ly.canon1, ly.canon_state1, h_ready, st));
     SEQ_TRY(front_product(m, ws, s, pend, ly.proj, ws->proj, 0, 0.f, 0.f, &done, st));
     if (!done) SEQ_TRY(lin(ly.proj, ws->proj, ws->h, T, 0, dt, st));
+    SEQ_TRY(adapt(ad, adapter_of(ad, &UmbSeqAdapters::proj, l), ly.proj, ws->proj, ws->h, T, dt, st));
     SEQ_TRY(run_mixer(m, ly, ws, s, st));
-    SEQ_TRY(lin_y(ly.out, ws->y, ws, ws->mix, T, ly.has_mlp ? slabs(ly.norm2, ly.canon2) : slabs(next_norm(l + 1), nl ? nl->canon1 : nullptr), dt, st));
+    const UmbSeqAdapter* const out_ad = adapter_of(ad, &UmbSeqAdapters::out, l);
+    int* const out_parts = ly.has_mlp ? slabs(ly.norm2, ly.canon2) : slabs(next_norm(l + 1), nl ? nl->canon1 : nullptr);
+    SEQ_TRY(lin_y(ly.out, ws->y, ws, ws->mix, T, out_ad && out_ad->a ? nullptr : out_parts, dt, st));
+    SEQ_TRY(adapt(ad, out_ad, ly.out, ws->y, ws->mix, T, dt, st));
     if (hyper) {
       // write of this sublayer and read of the next one (the feed-forward, the next layer's mixer, or nothing) in one launch
       const float* in2 = ly.has_mlp ? ly.hc2_in : (nl ? nl->hc1_in : nullptr);
@@ -715,6 +729,13 @@ extern "C" int umb_seq_forward(const UmbSeqModel* m, const UmbSeqWork* given, co
     SEQ_TRY(head_product(m, ws, s, st));
   }
   return UMB_OK;
+}
+
+extern "C" int umb_seq_forward(const UmbSeqModel* m, const UmbSeqWork* ws, const UmbSeqStep* s, hipStream_t st) { return forward(m, ws, s, nullptr, st); }
+
+extern "C" int umb_seq_forward_adapters(const UmbSeqModel* m, const UmbSeqWork* ws, const UmbSeqStep* s, const UmbSeqAdapters* ad, hipStream_t st) {
+  if (!ad || !ad->adapter || !ad->scratch || ad->S < 1) return UMB_EINVAL;
+  return forward(m, ws, s, ad, st);
 }
 
 extern "C" const char* umb_seq_version(void) { return "umbrella_seq 0.1 (gfx950)"; }

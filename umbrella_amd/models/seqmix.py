@@ -30,8 +30,9 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .._lib import UmbSeqLayer, UmbSeqLinear, UmbSeqModel, UmbSeqStep, UmbSeqWork
+from .._lib import UmbSeqAdapter, UmbSeqAdapters, UmbSeqLayer, UmbSeqLinear, UmbSeqModel, UmbSeqStep, UmbSeqWork
 from ..attn.cache import PagedSeqCache, send
+from .adapters import stack_adapters
 from .base import LLMBase
 from .config import SeqMixCfg, rotary_frequencies, rotary_table
 
@@ -477,9 +478,59 @@ class SeqMixLM(LLMBase):
     def logits_buffer(self) -> torch.Tensor:
         return self._bufs["logits"]
 
+    # ------------------------------------------------------------------ adapters
+    n_adapters = 0
+
+    def load_adapters(self, adapters):
+        """Low-rank adapters that sequences may name (``open(seq_id, adapter=i)``), beside the layers' input and output products.  adapters: one dict
+        each, ``{(layer, "proj" | "out"): (A [r, K], B [N, r], scale)}``, K and N those of the layer's product as it is run here (the mixer's projections
+        stacked in one); layers that an adapter does not name stay as they are.  An empty list takes them all away again."""
+        if any("adapter" in s for s in self.kv_cache.seqs.values()):
+            raise RuntimeError("adapters cannot be changed while open sequences run with one")
+        L, S, dev, dt = len(self.config.layers), len(adapters), torch.device(self.device), self.dtype
+        stacks, structs = {}, {}
+        for what in ("proj", "out"):
+            structs[what] = (UmbSeqAdapter * L)()
+            for i in range(L):
+                each = [a.get((i, what)) for a in adapters]
+                if not any(e is not None for e in each):
+                    continue
+                lin = getattr(self._layer_structs[i], what)
+                for e in each:
+                    if e is not None and (e[0].shape[1] != lin.K or e[1].shape[0] != lin.N):
+                        raise ValueError(f"layer {i}, {what}: A [r, {lin.K}] and B [{lin.N}, r] are wanted, got {tuple(e[0].shape)} and {tuple(e[1].shape)}")
+                none = (torch.zeros(1, lin.K), torch.zeros(lin.N, 1), 0.0)
+                a, b, scale, rank = stack_adapters([e or none for e in each], device=dev, dtype=dt)
+                rank *= torch.tensor([e is not None for e in each], dtype=torch.int32, device=dev)
+                stacks[i, what] = a, b, scale, rank
+                t = structs[what][i]
+                t.a, t.b, t.scale, t.rank, t.R = a.data_ptr(), b.data_ptr(), scale.data_ptr(), rank.data_ptr(), a.shape[1]
+        known = {(i, what) for i in range(L) for what in ("proj", "out")}
+        for n, a in enumerate(adapters):
+            if set(a) - known:
+                raise ValueError(f"adapter {n}: no such product: {sorted(set(a) - known, key=str)}")
+        self.n_adapters, self._adapter_stacks, self._adapter_structs = S, stacks, structs
+
+    def _adapter_struct(self, ids_ptr: int, T: int):
+        """the step's adapters, and the scratch that has to live until its launches are made"""
+        lib, most = _lib.load_seq(), 1
+        for (i, what), (a, *_) in self._adapter_stacks.items():
+            most = max(most, lib.umb_seq_adapters_floats(T, a.shape[2], a.shape[1]))
+        room = torch.empty(most, dtype=torch.float32, device=self.device)
+        ad = UmbSeqAdapters()
+        ad.proj, ad.out = (C.cast(self._adapter_structs[w], C.POINTER(UmbSeqAdapter)) for w in ("proj", "out"))
+        ad.adapter, ad.scratch, ad.scratch_floats, ad.S = ids_ptr, room.data_ptr(), most, self.n_adapters
+        return ad, room
+
     # ------------------------------------------------------------------ sequences
-    def open(self, seq_id):
-        return self.kv_cache.open(seq_id)
+    def open(self, seq_id, adapter: int | None = None):
+        """a slot for a new sequence, whose tokens run beside one of the loaded adapters, or none"""
+        if adapter is not None and not 0 <= adapter < self.n_adapters:
+            raise ValueError(f"the model has {self.n_adapters} adapters, got number {adapter}")
+        slot = self.kv_cache.open(seq_id)
+        if adapter is not None:
+            self.kv_cache.seqs[seq_id]["adapter"] = int(adapter)
+        return slot
 
     def close(self, seq_id):
         self.kv_cache.close(seq_id)
@@ -515,6 +566,10 @@ class SeqMixLM(LLMBase):
         if len(set(seq_slot)) < len(parts):          # a sequence named again: its parts are one stretch, whose rows stand together
             toks, first, back, (seq_slot, row0, pos0, lens) = _one_stretch_each(toks, seq_slot, row0, pos0, lens)
         T, B, R = len(toks), len(lens), len(rows)
+        # an adapter per row, where a sequence of the step names one
+        named = {s["slot"]: s["adapter"] for s in cache.seqs.values() if "adapter" in s} if self.n_adapters else {}
+        of_seq = [named.get(sl, -1) for sl in seq_slot]
+        adapted = any(a >= 0 for a in of_seq)
         self.reserve(T, max(R, 1))
         # tokens, their positions and slots | per sequence: slot, first row, first position, length | rows whose logits are wanted.  Sent without
         # waiting -- a copy that waits for the stream leaves the device idle while the host makes the step's launches, and a step's host work
@@ -531,7 +586,9 @@ class SeqMixLM(LLMBase):
             wanted = np.asarray(rows, dtype=np.int64) + np.repeat(np.asarray(first), counts)
             at[3 * T + 4 * B:] = wanted
             every = R == T and bool((wanted == np.arange(T)).all())         # every row, in order: the last seam norms them for the head
-        graphed = self.use_graph and not trace and T == B and str(dev).startswith("cuda")     # a pure decode step
+        if adapted:
+            meta_host = torch.cat([meta_host, torch.tensor(np.repeat(np.asarray(of_seq, dtype=np.int32), lens))])
+        graphed = self.use_graph and not trace and not adapted and T == B and str(dev).startswith("cuda")     # a pure decode step
         key = (T, R, every)
         if graphed:
             entry = self._graphs.get(key)
@@ -551,9 +608,13 @@ class SeqMixLM(LLMBase):
         tr = torch.empty(len(self.config.layers), T, self.config.width, dtype=torch.float32, device=dev) if trace else None
         s.trace = tr.data_ptr() if trace else None
         self._keep = meta
+        ad, room = self._adapter_struct(p + 4 * (meta_host.numel() - T), T) if adapted else (None, None)
 
         def launch():
-            rc = _lib.load_seq().umb_seq_forward(C.byref(self._m), C.byref(self._ws), C.byref(s), _lib.stream_ptr())
+            if adapted:
+                rc = _lib.load_seq().umb_seq_forward_adapters(C.byref(self._m), C.byref(self._ws), C.byref(s), C.byref(ad), _lib.stream_ptr())
+            else:
+                rc = _lib.load_seq().umb_seq_forward(C.byref(self._m), C.byref(self._ws), C.byref(s), _lib.stream_ptr())
             if rc != 0:
                 raise _lib.UmbError(f"libumbrella_seq umb_seq_forward failed with code {rc}")
         if graphed and entry["graph"] is not None:

@@ -14,10 +14,13 @@ tokens (trace replay): it owns the page / slot bookkeeping and calls the model's
 It keeps the engine surface (speculation/base.py) so the front-ends work unchanged: ``prefill`` / ``append`` /
 ``speculative_decoding`` drive one conversation (a tree of size one: ``build_tree`` has nothing to build, ``verify`` is a
 plain decode step), ``generate`` / ``generate_stream`` answer one API request, ``generate_batch`` many.
-Sampling uses the same device kernels as the speculation engines (arg-max, or penalty / top-k / temperature / top-p).
+Sampling uses the same device kernels as the speculation engines (arg-max, or penalty / top-k / temperature / top-p) where the engine's
+settings hold for all; a request may bring its own (``Sampling``: temperature, top-k, top-p, min-p, seed), ask for several continuations of
+its prompt (prefilled once, then forked: they share its full cache pages) and name a low-rank adapter of the model.
 """
 from __future__ import annotations
 
+import random
 import time
 from collections import deque
 from dataclasses import dataclass, field
@@ -25,13 +28,25 @@ from dataclasses import dataclass, field
 import torch
 
 from .. import _lib
+from ..attn.cache import send
 from ..logging_config import setup_logger
 from ..models import AutoModelLM
 from ..utils import TextColors
 from .base import BaseEngine
+from .sampling import sample_rows
 from .speculation_utils import IdTokenizer, is_sentence_complete_regex
 
 logger = setup_logger()
+
+
+@dataclass
+class Sampling:
+    """a request's own settings; a temperature of 0 is greedy, top_k 0 keeps all (include/umbrella_seq.h, umb_sample_requests)"""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: int = 0
 
 
 @dataclass
@@ -43,6 +58,10 @@ class Request:
     done: bool = False
     pending: int | None = None          # sampled, not yet fed through the model
     recorded: int = 0                   # tokens written to the device-side history of its slot
+    sampling: Sampling | None = None    # None: the engine's
+    rng: random.Random | None = None
+    adapter: int | None = None          # one of the model's
+    copies: list = field(default_factory=list)       # further continuations of the same prompt
 
 
 class BatchEngine(BaseEngine):
@@ -127,8 +146,29 @@ class BatchEngine(BaseEngine):
     def _greedy(self):
         return self.temperature < 0.05 and not (self.repetition_penalty > 1.01)
 
+    def _sample_own(self, logits, reqs):
+        """each row by its request's settings, or by the engine's where it has none, from its own random numbers"""
+        R = len(reqs)
+        if any(r.sampling is None for r in reqs) and self.repetition_penalty > 1.01:
+            raise ValueError("a repetition penalty does not go with requests that have settings of their own in the batch")
+        mine = [r.sampling or Sampling(0.0 if self.temperature < 0.05 else self.temperature, int(self.topk), float(self.topp)) for r in reqs]
+        for r in reqs:
+            if r.rng is None:
+                r.rng = random.Random(f"{r.sampling.seed if r.sampling else self.seed}/{r.id}")
+        host = torch.tensor([[s.temperature for s in mine], [s.top_p for s in mine], [s.min_p for s in mine], [r.rng.random() for r in reqs]], dtype=torch.float32)
+        both = send(torch.cat([host.view(torch.int32), torch.tensor([[s.top_k for s in mine]], dtype=torch.int32)]), self.device)
+        f = both.view(torch.float32)
+        tokens, _ = sample_rows(logits[:R], f[3], temperature=f[0], top_k=both[4], top_p=f[1], min_p=f[2])
+        tokens = tokens.tolist()
+        for r, t in zip(reqs, tokens):
+            if t < 0:
+                raise RuntimeError(f"request {r.id!r}: its logits leave no token to draw")
+        return tokens
+
     def _sample(self, logits, reqs):
         """one token per logits row (row i belongs to reqs[i]) -> list of ints"""
+        if any(r.sampling is not None for r in reqs):
+            return self._sample_own(logits, reqs)
         R = logits.shape[0]
         out = self.sampled[:R]
         if self._greedy():
@@ -159,30 +199,50 @@ class BatchEngine(BaseEngine):
         self.hist_len[slot] = req.recorded - 1             # the kernel reads indices 0 .. n inclusive
 
     # ------------------------------------------------------------------ scheduler
-    def submit(self, input_ids, max_new_tokens: int = 128, request_id=None):
+    def submit(self, input_ids, max_new_tokens: int = 128, request_id=None, sampling: Sampling | None = None, n: int = 1, adapter: int | None = None):
+        """Queues a request.  n > 1: so many continuations of the prompt; the further ones are requests (request_id, 1) to (request_id, n - 1) of
+        their own, each with random numbers of its own."""
         ids = [int(t) for t in (input_ids.reshape(-1).tolist() if isinstance(input_ids, torch.Tensor) else input_ids)]
         if not ids:
             raise ValueError("a request needs at least one prompt token")
         if len(ids) + max_new_tokens > self.max_length:
             raise ValueError(f"prompt ({len(ids)}) + max_new_tokens ({max_new_tokens}) exceeds max_length {self.max_length}")
+        if sampling is not None and self.repetition_penalty > 1.01:
+            raise ValueError("a repetition penalty does not go with settings of a request's own")
+        if not 1 <= n <= self.max_batch:
+            raise ValueError(f"1 to {self.max_batch} continuations (sequence slots) are possible, got {n}")
+        if adapter is not None and not 0 <= adapter < getattr(self.target_model, "n_adapters", 0):
+            raise ValueError(f"the model has {getattr(self.target_model, 'n_adapters', 0)} adapters, got number {adapter}")
         if request_id is None:
             request_id, self._next_id = self._next_id, self._next_id + 1
-        self.queue.append(Request(request_id, ids, int(max_new_tokens)))
+        r = Request(request_id, ids, int(max_new_tokens), sampling=sampling, adapter=adapter)
+        r.copies = [Request((request_id, i), ids, int(max_new_tokens), sampling=sampling, adapter=adapter) for i in range(1, n)]
+        self.queue.append(r)
         return request_id
+
+    def _pages_wanted(self, r) -> int:
+        """pages that a request and its further continuations may come to hold"""
+        page = self.target_model.kv_cache.page
+        whole, shared = (len(r.prompt) + r.max_new_tokens + page - 1) // page, len(r.prompt) // page
+        return whole + len(r.copies) * (whole - shared)
 
     def _admit(self):
         """static batching: called only when nothing runs; first come first served while slots and pages last"""
         cache = self.target_model.kv_cache
         budget = len(cache.free_pages)
-        while self.queue and len(self.running) < self.max_batch and len(cache.free_slots) > len(self.running):
+        slots = 0
+        while self.queue and slots + len(self.queue[0].copies) < min(self.max_batch, len(cache.free_slots)):
             r = self.queue[0]
-            need = (len(r.prompt) + r.max_new_tokens + cache.page - 1) // cache.page
+            need = self._pages_wanted(r)
             if need > budget:
                 if not self.running:
                     raise RuntimeError(f"request {r.id!r} needs {need} cache pages, the cache has {budget} free")
                 break
             budget -= need
+            slots += 1 + len(r.copies)
             self.running.append(self.queue.popleft())
+        if not self.running and self.queue and self.queue[0].copies:
+            raise RuntimeError(f"request {self.queue[0].id!r} needs {1 + len(self.queue[0].copies)} sequence slots, {len(cache.free_slots)} are free")
 
     def _retire(self, r):
         r.done = True
@@ -200,12 +260,17 @@ class BatchEngine(BaseEngine):
             batch = list(self.running)
             entries = [(r.id, r.prompt, [len(r.prompt) - 1]) for r in batch]
             for r in batch:
-                self.target_model.open(r.id)
+                if r.adapter is None:
+                    self.target_model.open(r.id)
+                else:
+                    self.target_model.open(r.id, adapter=r.adapter)
                 self._record(r, r.prompt)
         else:
             batch = list(self.running)
             entries = [(r.id, [r.pending], [0]) for r in batch]
         logits = self.run_step(entries)
+        if any(r.copies for r in batch):
+            batch, logits = self._branch(batch, logits)
         new = self._sample(logits, batch)
         end = []
         for r, tok in zip(batch, new):
@@ -219,13 +284,33 @@ class BatchEngine(BaseEngine):
             self._retire(r)
         return bool(self.running or self.queue)
 
+    def _branch(self, batch, logits):
+        """behind the prompts' step: the further continuations of each go on from its sequence, and from its logits"""
+        row, out = [], []
+        for i, r in enumerate(batch):
+            self.target_model.kv_cache.fork(r.id, [c.id for c in r.copies])
+            for c in r.copies:
+                self._record(c, c.prompt)
+            row += [i] * (1 + len(r.copies))
+            out += [r, *r.copies]
+            r.copies = []
+        self.running = list(out)
+        return out, logits[send(torch.tensor(row, dtype=torch.long), logits.device)]
+
     @torch.inference_mode()
-    def generate_batch(self, prompts, max_new_tokens: int = 128):
-        """prompts: list of token-id lists -> list of generated token-id lists (greedy or sampled per the engine's knobs)"""
-        ids = [self.submit(p, max_new_tokens) for p in prompts]
+    def generate_batch(self, prompts, max_new_tokens: int = 128, sampling=None, n: int = 1, adapters=None):
+        """prompts: list of token-id lists -> list of generated token-id lists (greedy or sampled per the engine's knobs).  sampling: one
+        ``Sampling`` for all, or one (or None) per prompt; adapters: a number (or None) per prompt; n > 1: a list of n continuations per prompt."""
+        each = list(sampling) if isinstance(sampling, (list, tuple)) else [sampling] * len(prompts)
+        named = list(adapters) if adapters is not None else [None] * len(prompts)
+        if len(each) != len(prompts) or len(named) != len(prompts):
+            raise ValueError("settings and adapters: one per prompt")
+        ids = [self.submit(p, max_new_tokens, sampling=s, n=n, adapter=a) for p, s, a in zip(prompts, each, named)]
         while self.step():
             pass
-        return [self.finished.pop(i).generated for i in ids]
+        if n == 1:
+            return [self.finished.pop(i).generated for i in ids]
+        return [[self.finished.pop(i if k == 0 else (i, k)).generated for k in range(n)] for i in ids]
 
     # ------------------------------------------------------------------ one conversation (engine surface)
     def prefill(self, text: str):
@@ -317,6 +402,12 @@ class BatchEngine(BaseEngine):
         self.seed = seed
         self.rng_state.fill_(seed)
 
+    def _api_sampling(self, api_args):
+        """an API request that names min_p has settings of its own; others run by the engine's"""
+        if api_args.get("min_p") is None:
+            return None
+        return Sampling(0.0 if self.temperature < 0.05 else float(self.temperature), int(self.topk), float(self.topp), float(api_args["min_p"]), int(api_args.get("seed", self.seed)))
+
     def _request_ids(self, api_args):
         input_ids = api_args.get("input_ids", None)
         if input_ids is None:
@@ -335,7 +426,7 @@ class BatchEngine(BaseEngine):
             return api_args
         torch.cuda.synchronize()
         t1 = time.time()
-        toks = self.generate_batch([ids], n)[0]
+        toks = self.generate_batch([ids], n, sampling=self._api_sampling(api_args))[0]
         torch.cuda.synchronize()
         t2 = time.time()
         api_args["generated_text"] = self.tokenizer.decode(toks, skip_special_tokens=True, clean_up_tokenization_spaces=False)
@@ -353,7 +444,7 @@ class BatchEngine(BaseEngine):
         if len(ids) + n > self.max_length:
             yield "Exceeding reserved allowed context length", "Exceeding reserved allowed context length"
             return
-        rid = self.submit(ids, n)
+        rid = self.submit(ids, n, sampling=self._api_sampling(api_args))
         t1, text = time.time(), ""
         while self.step():
             r = next((q for q in self.running if q.id == rid), None)
