@@ -62,6 +62,13 @@ def test_pages_of_many_pieces():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("groups,rows,row,per", [(1 << 23, 2, 1, 1), (1 << 21, 3, 2, 1), (3000001, 3, 1, 1), ((1 << 22) - 1, 2, 1, 1), (70001, 50, 4, 7)])
+def test_pages_of_very_many_groups(groups, rows, row, per):
+    """a row a group: more groups than a fraction of 24 bits tells apart"""
+    check([(4, groups, rows, row, torch.uint8, per)], [(0, 2, 1), (3, 1, rows * per - 1)])
+
+
+@pytest.mark.gpu
 def test_many_moves():
     """more than a grid's rows"""
     n = 70000
