@@ -70,63 +70,49 @@ template <int TILE> __device__ __forceinline__ Tile tile_of_row(int t, int T, in
 }
 
 // More rows: plan, of each window: how many tiles; their adapters; their first places and sizes (first + 1024 n); the window's rows, those of a tile side by
-// side.  A quarter of the window's rows is compared with each row by one of four threads.
+// side.  A wave a window, four rows a lane: adapter by adapter, in the order of their first rows, whose rows are found by comparisons and placed by counting
+// bits.  (All rows against all by 1024 threads took 7.6 us whatever there was; this 4 where a window has a few adapters.)
 constexpr int PLAN_TILE = 64, PLAN_INTS = 1 + 3 * WINDOW;
-__global__ __launch_bounds__(4 * WINDOW) void adapter_plan_kernel(int* __restrict__ plan, const int* __restrict__ adapter, int T, int S) {
-  __shared__ __attribute__((aligned(16))) int ids[WINDOW], firsts[WINDOW];
-  __shared__ int said[4][3][WINDOW], waves[4];
-  const int i = threadIdx.x % WINDOW, q = threadIdx.x / WINDOW, t = blockIdx.x * WINDOW + i, lane = i & 63, wave = i >> 6;
+__global__ __launch_bounds__(64) void adapter_plan_kernel(int* __restrict__ plan, const int* __restrict__ adapter, int T, int S) {
+  constexpr int NE = WINDOW / 64;
+  const int lane = threadIdx.x, t0 = blockIdx.x * WINDOW;
   int* p = plan + (long)blockIdx.x * PLAN_INTS;
-  int id = t < T ? adapter[t] : -2;
-  if (t < T && (id < 0 || id >= S)) id = -1;
-  if (q == 0) ids[i] = id;
-  __syncthreads();
-  int at = 0, n = 0, first = WINDOW;         // the row's place among its adapter's, how many those are, the first of them
-#pragma unroll 4
-  for (int j0 = (q + 1) * (WINDOW / 4) - 4; j0 >= q * (WINDOW / 4); j0 -= 4) {
-    const int4 v = *reinterpret_cast<const int4*>(ids + j0);
-    const int o[4] = {v.x, v.y, v.z, v.w};
+  int id[NE];
+  unsigned long long left[NE];
 #pragma unroll
-    for (int e = 3; e >= 0; --e) {
-      const bool same = o[e] == id;
-      n += same;
-      at += same && j0 + e < i;
-      first = same ? j0 + e : first;
+  for (int e = 0; e < NE; ++e) {
+    const int t = t0 + 64 * e + lane;
+    id[e] = t < T ? adapter[t] : -2;
+    if (t < T && (id[e] < 0 || id[e] >= S)) id[e] = -1;
+  }
+#pragma unroll
+  for (int e = 0; e < NE; ++e) left[e] = __ballot(id[e] != -2);
+  const unsigned long long below = (1ull << lane) - 1ull;
+  int tiles = 0, front = 0;
+  for (;;) {
+    int mine = -2;
+#pragma unroll
+    for (int e = NE - 1; e >= 0; --e)
+      if (left[e]) mine = __builtin_amdgcn_readlane(id[e], __ffsll(left[e]) - 1);
+    if (mine == -2) break;
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const bool same = id[e] == mine;
+      const unsigned long long bal = __ballot(same);
+      if (same) p[1 + 2 * WINDOW + front + n + __popcll(bal & below)] = t0 + 64 * e + lane;
+      n += __popcll(bal);
+      left[e] &= ~bal;
     }
+    const int k = (n + PLAN_TILE - 1) / PLAN_TILE;
+    if (lane < k) {
+      p[1 + tiles + lane] = mine;
+      p[1 + WINDOW + tiles + lane] = front + lane * PLAN_TILE + 1024 * min(PLAN_TILE, n - lane * PLAN_TILE);
+    }
+    tiles += k;
+    front += n;
   }
-  said[q][0][i] = at;
-  said[q][1][i] = n;
-  said[q][2][i] = first;
-  __syncthreads();
-  at = n = 0;
-  first = WINDOW;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) { at += said[k][0][i]; n += said[k][1][i]; first = min(first, said[k][2][i]); }
-  if (q == 0) firsts[i] = first;
-  __syncthreads();
-  // rows of an adapter stand together, adapters in the order of their first rows: in front of this row's are those whose first row is an earlier one
-  int front = 0;
-#pragma unroll 4
-  for (int j0 = q * (WINDOW / 4); j0 < (q + 1) * (WINDOW / 4); j0 += 4) {
-    const int4 v = *reinterpret_cast<const int4*>(firsts + j0);
-    front += (v.x < first) + (v.y < first) + (v.z < first) + (v.w < first);
-  }
-  said[q][0][i] = front;                     // (at is read by now: firsts stands between)
-  const bool leads = id != -2 && at % PLAN_TILE == 0;
-  const unsigned long long bal = __ballot(leads);
-  if (q == 0 && lane == 0) waves[wave] = __popcll(bal);
-  __syncthreads();
-  if (q > 0) return;
-  front = said[0][0][i] + said[1][0][i] + said[2][0][i] + said[3][0][i];
-  int k = __popcll(bal & ((1ull << lane) - 1ull)), all = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) { if (w < wave) k += waves[w]; all += waves[w]; }
-  if (i == 0) p[0] = all;
-  if (leads) {
-    p[1 + k] = id;
-    p[1 + WINDOW + k] = front + at + 1024 * min(PLAN_TILE, n - at);
-  }
-  if (id != -2) p[1 + 2 * WINDOW + front + at] = t;
+  if (lane == 0) p[0] = tiles;
 }
 __device__ __forceinline__ Tile tile_of_plan(const int* __restrict__ p, int k, int* rows) {
   const int said = p[1 + WINDOW + k], n = said / 1024, first = said % 1024;
@@ -151,7 +137,7 @@ __device__ __forceinline__ void each_tile(const int* plan, int slots, int T, int
 
 // ---- u[part][t][r] = sum over the part's K of A x.  grid (parts, rows or slots: the parts fastest, since blocks go round the eight dies and of a window's slots the first few alone have tiles).  Stages of KB bytes of K, of 16 TF tokens and 16 RF ranks, go through
 // registers to LDS, the next stage's loads in flight behind this one's products.  TF 4: a wave 16 of the tokens; 1: a quarter of the stage's K.
-template <typename P, bool WHOLE, int RF, int TF, int KB>
+template <typename P, bool WHOLE, int RF, int TF, int KB, int AHEAD>
 __global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u, const typename El<P>::type* __restrict__ x, const typename El<P>::type* __restrict__ a,
                                                            const int* __restrict__ adapter, const int* __restrict__ rank, const int* __restrict__ plan, int slots,
                                                            int T, int K, int S, int R, int per) {
@@ -169,9 +155,9 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u
     const int ra = rank ? min(max(rank[tile.adapter], 0), R) : R;
     if (ra < 1) return;
     const E* ap = a + (long)tile.adapter * R * K;
-    u32x4 xv[NX], av[NA];
+    u32x4 xs[AHEAD][NX], as[AHEAD][NA];
     // rows that are not there are zeros
-    auto load = [&](int k) __attribute__((always_inline)) {
+    auto load = [&](u32x4 (&xv)[NX], u32x4 (&av)[NA], int k) __attribute__((always_inline)) {
       const int at = k + piece * VE, left = k1 - at;
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
@@ -188,16 +174,15 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u
     f32x4 acc[RF];
 #pragma unroll
     for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    load(k0);
-    for (int k = k0; k < k1; k += KC) {
+    auto step = [&](u32x4 (&xv)[NX], u32x4 (&av)[NA], int k) __attribute__((always_inline)) {
       if (k > k0) __syncthreads();           // (the stage before this one has been read)
 #pragma unroll
       for (int i = 0; i < NX; ++i) *reinterpret_cast<u32x4*>(stage + (row + i * ROWS) * LD + piece * 16) = xv[i];
 #pragma unroll
       for (int i = 0; i < NA; ++i) *reinterpret_cast<u32x4*>(stage + (16 * TF + row + i * ROWS) * LD + piece * 16) = av[i];
       __syncthreads();
-      if (k + KC < k1) load(k + KC);
-      if (TF == 4 && wave * 16 >= tile.n) continue;
+      if (k + AHEAD * KC < k1) load(xv, av, k + AHEAD * KC);
+      if (TF == 4 && wave * 16 >= tile.n) return;
       constexpr int MINE = TF == 4 ? STEPS : STEPS / 4;
 #pragma unroll
       for (int s0 = 0; s0 < MINE; ++s0) {
@@ -208,7 +193,12 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u
         for (int f = 0; f < RF; ++f)
           if (16 * f < ra) acc[f] = mma<P>(*reinterpret_cast<const Frag<P>*>(at + (16 * TF + 16 * f) * LD), b, acc[f]);
       }
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) if (k0 + i * KC < k1 || i == 0) load(xs[i], as[i], k0 + i * KC);
+    for (int k = k0; k < k1; k += AHEAD * KC)
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) if (k + i * KC < k1) step(xs[i], as[i], k + i * KC);
     if constexpr (TF == 1) {
       __syncthreads();
       f32x4(*part)[RF][64] = reinterpret_cast<f32x4(*)[RF][64]>(stage);
@@ -404,7 +394,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float
         const int r = row + i * ROWS, col = n + 4 * quad;
         if (r >= tile.n) continue;
         float* o = out + (long)rows[r] * N + col;
-        if (QUADS) { if (col < n1) *reinterpret_cast<f32x4*>(o) = y[i]; }
+        if (QUADS) { if (col < n1) __builtin_nontemporal_store(y[i], reinterpret_cast<f32x4*>(o)); }
         else
 #pragma unroll
           for (int e = 0; e < 4; ++e) if (col + e < n1) o[e] = y[i][e];
@@ -414,7 +404,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float
   });
 }
 
-static int adapter_parts(int T, int K) { return std::max(1, std::min(T > 4096 ? 4 : 8, (K + 511) / 512)); }
+static int adapter_parts(int T, int K) { return std::max(1, std::min(T > 4096 ? 2 : T > 2048 ? 4 : 8, (K + 511) / 512)); }
 static long plan_ints(int T) { return T > WINDOW ? (long)((T + WINDOW - 1) / WINDOW) * PLAN_INTS : 0; }
 
 extern "C" long umb_seq_adapters_floats(int T, int K, int R) {
@@ -434,17 +424,17 @@ static int adapters_launch(float* out, const float* base, const void* x, const v
     slots = T <= 2048 ? 32 : 8;
     blocks = windows * slots;
     tiles = (T + PLAN_TILE - 1) / PLAN_TILE;
-    hipLaunchKernelGGL(adapter_plan_kernel, dim3(windows), dim3(4 * WINDOW), 0, st, plan, adapter, T, S);
+    hipLaunchKernelGGL(adapter_plan_kernel, dim3(windows), dim3(64), 0, st, plan, adapter, T, S);
     UMB_LAUNCH_CHECK();
   }
-#define DOWN(RF, KB)                                                                                                                                       \
-  hipLaunchKernelGGL((adapter_down_kernel<P, WHOLE, RF, TF, KB>), dim3(parts, blocks), dim3(256), 0, st, u, (const E*)x, (const E*)a, adapter, rank, plan, slots, \
+#define DOWN(RF, KB, AHEAD)                                                                                                                                       \
+  hipLaunchKernelGGL((adapter_down_kernel<P, WHOLE, RF, TF, KB, AHEAD>), dim3(parts, blocks), dim3(256), 0, st, u, (const E*)x, (const E*)a, adapter, rank, plan, slots, \
                      T, K, S, R, per)
-  // bytes of K a stage: 8 to 12 loads a thread in flight, and for few tokens the least stages
-  if (R <= 16) DOWN(1, (TF == 1 ? 1024 : 512));
-  else if (R <= 32) DOWN(2, 512);
-  else if (R <= 64) DOWN(4, (TF == 1 ? 512 : 256));
-  else DOWN(8, (TF == 1 && !std::is_same_v<P, F32> ? 256 : TF == 1 ? 512 : 256));
+  // bytes of K a stage, and stages in flight
+  if (R <= 16) DOWN(1, (TF == 1 ? 1024 : 512), (TF == 1 ? 1 : 2));
+  else if (R <= 32) DOWN(2, 512, (TF == 1 ? 1 : 2));
+  else if (R <= 64) DOWN(4, (TF == 1 ? 512 : 256), (TF == 1 ? 1 : 2));
+  else DOWN(8, (TF == 1 && !std::is_same_v<P, F32> ? 256 : TF == 1 ? 512 : 256), 1);
 #undef DOWN
   UMB_LAUNCH_CHECK();
   int columns = 256;
