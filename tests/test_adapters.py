@@ -83,6 +83,15 @@ def test_widths(name, K, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("R,K", [(8, 4096), (8, 4104), (16, 2048), (32, 1024), (33, 990), (64, 512), (64, 520), (1, 32768), (1, 33000)])
+@pytest.mark.parametrize("T", [1, 5, 64, 65])
+def test_both_sides_of_one_launch(name, R, K, T):
+    """the sizes up to which both products are one launch, and just beyond"""
+    check(make(T, K, 300, 3, R, TYPES[name], seed=T, ids="any", ranks=[R, max(1, R - 3)]), inplace=T == 5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [255, 256, 257, 511, 700, 1025, 2049])
 @pytest.mark.parametrize("ids", ["runs", "any", "one"])
 def test_more_rows_than_a_window(T, ids):
@@ -229,10 +238,11 @@ def test_refusals_on_the_device():
 @pytest.mark.parametrize("kw", [dict(T=0), dict(N=0), dict(K=0), dict(S=0), dict(R=0), dict(R=129), dict(out=None), dict(base=None), dict(x=None), dict(a=None), dict(b=None),
                                 dict(adapter=None), dict(scratch=None), dict(scratch=AT + 4), dict(floats=-1), dict(dtype=3)])
 def test_refusals_of_the_entry_point(kw):
-    a = dict(T=4, N=8, K=16, S=2, R=8, out=AT, base=AT, x=AT, a=AT, b=AT, adapter=AT, scratch=AT, floats=0, dtype=1)
+    a = dict(T=100, N=8, K=16, S=2, R=8, out=AT, base=AT, x=AT, a=AT, b=AT, adapter=AT, scratch=AT, floats=0, dtype=1)
     a.update(kw)
     lib = _lib.load_seq()
-    n = lib.umb_seq_adapters_floats(4, 16, 8) + a["floats"]
+    n = lib.umb_seq_adapters_floats(100, 16, 8) + a["floats"]
     assert lib.umb_seq_adapters_floats(0, 8, 8) == 0 and lib.umb_seq_adapters_floats(8, 0, 8) == 0 and lib.umb_seq_adapters_floats(8, 8, 129) == 0
+    assert lib.umb_seq_adapters_floats(100, 16, 8) > 0 and lib.umb_seq_adapters_floats(4, 16, 8) == 0        # few tokens: one launch, no scratch
     assert lib.umb_seq_adapters(a["out"], a["base"], a["x"], a["a"], a["b"], a["adapter"], None, None, a["T"], a["N"], a["K"], a["S"], a["R"], a["scratch"], n, a["dtype"],
                                 None) == EINVAL

@@ -3,12 +3,13 @@
 // x [T][K], A [S][R][K], B [S][N][R] in `dtype`; base and out fp32 [T][N]; of adapter a the first rank[a] of R count.  A row whose number is none of
 // 0 .. S - 1 is its base.
 //
-// Two launches: u = A x, fp32, summed over K in `parts` pieces; then out.  Rows of one adapter are taken together, so that A and B are read once for them.
+// Two launches (one where the factors are small): u = A x, fp32, summed over K in `parts` pieces; then out.  Rows of one adapter are taken together, so that A and B are read once for them.
 // Up to 256 rows: tiles of 16; the row whose place among its adapter's rows is a multiple of 16 stands for those from it on, and every other row's block is
 // empty: nothing is sorted or counted beforehand.  More rows: tiles of 64, and a launch in front works them out once for each window of 256.
 //
 // Bound by memory: x, A, B and the base are read once and out is written once, in pieces of 256 contiguous bytes and more, which fragments read from
-// memory directly (16 rows x 64 bytes) are not: they took 46 + 71 us where staging takes 10 + 16 (1999 tokens, fp16, 4096 x 4096, rank 32; 8192 tokens, bf16, 4096 x 6144, rank 64: 83 + 222, 30 + 107).
+// memory directly (16 rows x 64 bytes) are not: they took 46 + 71 us where
+// staging takes 9.6 + 15.8 (1999 tokens, fp16, 4096 x 4096, rank 32; 8192 tokens, bf16, 4096 x 6144, rank 64: 83 + 222, 30 + 99).
 //
 // u enters the second product with 22 bits or more: three bf16 terms (each the rest that the one before left), two fp16 ones behind a power of two per row
 // (whatever u's size), or itself in fp32.
@@ -135,84 +136,92 @@ __device__ __forceinline__ void each_tile(const int* plan, int slots, int T, int
   }
 }
 
-// ---- u[part][t][r] = sum over the part's K of A x.  grid (parts, rows or slots: the parts fastest, since blocks go round the eight dies and of a window's slots the first few alone have tiles).  Stages of KB bytes of K, of 16 TF tokens and 16 RF ranks, go through
-// registers to LDS, the next stage's loads in flight behind this one's products.  TF 4: a wave 16 of the tokens; 1: a quarter of the stage's K.
+// ---- A x of a tile over K's k0 .. k1.  Stages of KB bytes of K, of 16 TF tokens and 16 RF ranks, go through registers to LDS, the next AHEAD stages' loads in flight
+// behind this one's products.  TF 4: a wave 16 of the tokens; 1: a quarter of the stage's K, and wave 0 is left with the sums.
+template <typename P, int RF, int TF, int KB> struct Down {
+  typedef typename El<P>::type E;
+  static constexpr int ES = sizeof(E), KC = KB / ES, VE = 16 / ES, LD = KB + 16, STEPS = KC / 32, PER_ROW = KB / 16, ROWS = 256 / PER_ROW;
+  static constexpr int NX = 16 * TF / ROWS > 0 ? 16 * TF / ROWS : 1, NA = 16 * RF / ROWS > 0 ? 16 * RF / ROWS : 1, ROOM = (16 * TF + 16 * RF) * LD;
+  static_assert(16 % ROWS == 0 && (TF == 4 || STEPS % 4 == 0) && (TF == 4 || 3 * RF * 64 * 16 <= ROOM));
+};
+template <typename P, bool WHOLE, int RF, int TF, int KB, int AHEAD>
+__device__ __forceinline__ void down_sums(f32x4 (&acc)[RF], char* stage, const int* rows, Tile tile, int ra, const typename El<P>::type* __restrict__ x,
+                                          const typename El<P>::type* __restrict__ ap, int K, int k0, int k1) {
+  typedef Down<P, RF, TF, KB> D;
+  constexpr int NX = D::NX, NA = D::NA, LD = D::LD, KC = D::KC, ROWS = D::ROWS, VE = D::VE;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4, row = threadIdx.x / D::PER_ROW, piece = threadIdx.x % D::PER_ROW;
+  u32x4 xs[AHEAD][NX], as[AHEAD][NA];
+  // rows that are not there are zeros
+  auto load = [&](u32x4 (&xv)[NX], u32x4 (&av)[NA], int k) __attribute__((always_inline)) {
+    const int at = k + piece * VE, left = k1 - at;
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const int r = row + i * ROWS;
+      const bool in = r < tile.n;
+      xv[i] = load_some<P, WHOLE, u32x4, VE>(x + (long)rows[in ? r : 0] * K + at, in ? left : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int r = row + i * ROWS;
+      av[i] = load_some<P, WHOLE, u32x4, VE>(ap + (long)(r < ra ? r : 0) * K + at, r < ra ? left : 0);
+    }
+  };
+#pragma unroll
+  for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto step = [&](u32x4 (&xv)[NX], u32x4 (&av)[NA], int k) __attribute__((always_inline)) {
+    if (k > k0) __syncthreads();             // (the stage before this one has been read)
+#pragma unroll
+    for (int i = 0; i < NX; ++i) *reinterpret_cast<u32x4*>(stage + (row + i * ROWS) * LD + piece * 16) = xv[i];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) *reinterpret_cast<u32x4*>(stage + (16 * TF + row + i * ROWS) * LD + piece * 16) = av[i];
+    __syncthreads();
+    if (k + AHEAD * KC < k1) load(xv, av, k + AHEAD * KC);
+    // (all ranks and rows, zeros among them: with a branch between two products the compiler leaves too few cycles in front of the first one's sums)
+    constexpr int MINE = TF == 4 ? D::STEPS : D::STEPS / 4;
+#pragma unroll
+    for (int s0 = 0; s0 < MINE; ++s0) {
+      const int s = TF == 4 ? s0 : wave * MINE + s0;
+      const char* at = stage + j * LD + (32 * s + 8 * g) * D::ES;
+      const Frag<P> b = *reinterpret_cast<const Frag<P>*>(at + (TF == 4 ? wave * 16 * LD : 0));
+#pragma unroll
+      for (int f = 0; f < RF; ++f) acc[f] = mma<P>(*reinterpret_cast<const Frag<P>*>(at + (16 * TF + 16 * f) * LD), b, acc[f]);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) if (k0 + i * KC < k1 || i == 0) load(xs[i], as[i], k0 + i * KC);
+  for (int k = k0; k < k1; k += AHEAD * KC)
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) if (k + i * KC < k1) step(xs[i], as[i], k + i * KC);
+  if constexpr (TF == 1) {
+    __syncthreads();
+    f32x4(*part)[RF][64] = reinterpret_cast<f32x4(*)[RF][64]>(stage);
+    if (wave > 0)
+#pragma unroll
+      for (int f = 0; f < RF; ++f) part[wave - 1][f][lane] = acc[f];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int f = 0; f < RF; ++f) acc[f] = (acc[f] + part[0][f][lane]) + (part[1][f][lane] + part[2][f][lane]);
+  }
+}
+
+// u[part][t][r].  grid (parts, rows or slots: the parts fastest, since blocks go round the eight dies and of a window's slots the first few alone have tiles)
 template <typename P, bool WHOLE, int RF, int TF, int KB, int AHEAD>
 __global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u, const typename El<P>::type* __restrict__ x, const typename El<P>::type* __restrict__ a,
                                                            const int* __restrict__ adapter, const int* __restrict__ rank, const int* __restrict__ plan, int slots,
                                                            int T, int K, int S, int R, int per) {
-  typedef typename El<P>::type E;
-  constexpr int ES = sizeof(E), KC = KB / ES, VE = 16 / ES, LD = KB + 16, STEPS = KC / 32, PER_ROW = KB / 16, ROWS = 256 / PER_ROW;
-  constexpr int NX = 16 * TF / ROWS > 0 ? 16 * TF / ROWS : 1, NA = 16 * RF / ROWS > 0 ? 16 * RF / ROWS : 1;
-  static_assert(16 % ROWS == 0 && (TF == 4 || STEPS % 4 == 0));
   __shared__ int rows[16 * TF], waves[5];
-  __shared__ __attribute__((aligned(16))) char stage[(16 * TF + 16 * RF) * LD];
+  __shared__ __attribute__((aligned(16))) char stage[Down<P, RF, TF, KB>::ROOM];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int row = threadIdx.x / PER_ROW, piece = threadIdx.x % PER_ROW;
   const int k0 = blockIdx.x * per, k1 = min(K, k0 + per);
   each_tile<TF>(plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
     if (tile.adapter < 0) return;
     const int ra = rank ? min(max(rank[tile.adapter], 0), R) : R;
     if (ra < 1) return;
-    const E* ap = a + (long)tile.adapter * R * K;
-    u32x4 xs[AHEAD][NX], as[AHEAD][NA];
-    // rows that are not there are zeros
-    auto load = [&](u32x4 (&xv)[NX], u32x4 (&av)[NA], int k) __attribute__((always_inline)) {
-      const int at = k + piece * VE, left = k1 - at;
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const int r = row + i * ROWS;
-        const bool in = r < tile.n;
-        xv[i] = load_some<P, WHOLE, u32x4, VE>(x + (long)rows[in ? r : 0] * K + at, in ? left : 0);
-      }
-#pragma unroll
-      for (int i = 0; i < NA; ++i) {
-        const int r = row + i * ROWS;
-        av[i] = load_some<P, WHOLE, u32x4, VE>(ap + (long)(r < ra ? r : 0) * K + at, r < ra ? left : 0);
-      }
-    };
     f32x4 acc[RF];
-#pragma unroll
-    for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto step = [&](u32x4 (&xv)[NX], u32x4 (&av)[NA], int k) __attribute__((always_inline)) {
-      if (k > k0) __syncthreads();           // (the stage before this one has been read)
-#pragma unroll
-      for (int i = 0; i < NX; ++i) *reinterpret_cast<u32x4*>(stage + (row + i * ROWS) * LD + piece * 16) = xv[i];
-#pragma unroll
-      for (int i = 0; i < NA; ++i) *reinterpret_cast<u32x4*>(stage + (16 * TF + row + i * ROWS) * LD + piece * 16) = av[i];
-      __syncthreads();
-      if (k + AHEAD * KC < k1) load(xv, av, k + AHEAD * KC);
-      if (TF == 4 && wave * 16 >= tile.n) return;
-      constexpr int MINE = TF == 4 ? STEPS : STEPS / 4;
-#pragma unroll
-      for (int s0 = 0; s0 < MINE; ++s0) {
-        const int s = TF == 4 ? s0 : wave * MINE + s0;
-        const char* at = stage + j * LD + (32 * s + 8 * g) * ES;
-        const Frag<P> b = *reinterpret_cast<const Frag<P>*>(at + (TF == 4 ? wave * 16 * LD : 0));
-#pragma unroll
-        for (int f = 0; f < RF; ++f)
-          if (16 * f < ra) acc[f] = mma<P>(*reinterpret_cast<const Frag<P>*>(at + (16 * TF + 16 * f) * LD), b, acc[f]);
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) if (k0 + i * KC < k1 || i == 0) load(xs[i], as[i], k0 + i * KC);
-    for (int k = k0; k < k1; k += AHEAD * KC)
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) if (k + i * KC < k1) step(xs[i], as[i], k + i * KC);
-    if constexpr (TF == 1) {
-      __syncthreads();
-      f32x4(*part)[RF][64] = reinterpret_cast<f32x4(*)[RF][64]>(stage);
-      static_assert(3 * RF * 64 * 16 <= (16 + 16 * RF) * LD);
-      if (wave > 0)
-#pragma unroll
-        for (int f = 0; f < RF; ++f) part[wave - 1][f][lane] = acc[f];
-      __syncthreads();
-      if (wave > 0) return;
-#pragma unroll
-      for (int f = 0; f < RF; ++f) acc[f] = (acc[f] + part[0][f][lane]) + (part[1][f][lane] + part[2][f][lane]);
-    }
+    down_sums<P, WHOLE, RF, TF, KB, AHEAD>(acc, stage, rows, tile, ra, x, a + (long)tile.adapter * R * K, K, k0, k1);
     const int own = TF == 4 ? wave * 16 + j : j;
-    if (own >= tile.n) return;
+    if ((TF == 1 && wave > 0) || own >= tile.n) return;
     float* to = u + ((long)blockIdx.x * T + rows[own]) * R;
 #pragma unroll
     for (int f = 0; f < RF; ++f) {
@@ -225,17 +234,23 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u
   });
 }
 
-// ---- out = base + B (scale u).  grid (pieces of N, rows or slots).  Stages of CS columns: a wave's share of them for all the tile's rows goes to LDS, from where whole rows
+// ---- out = base + B (scale u).  grid (pieces of N, rows or slots).  RF > 0: u is worked out here too, once for each piece of N, from an A that is small enough for that.
+//  Stages of CS columns: a wave's share of them for all the tile's rows goes to LDS, from where whole rows
 // leave, joined by the base (asked for in front of everything else).
 template <typename P> struct Terms { static constexpr int N = 1; };
 template <> struct Terms<BF16> { static constexpr int N = 3; };
 template <> struct Terms<F16> { static constexpr int N = 2; };
 
-template <typename P, bool WHOLE, bool QUADS, int RC, int TF>
+template <typename P, bool WHOLE, bool QUADS, int RC, int TF, int RF, int KB>
 __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float* base, const float* __restrict__ u, const typename El<P>::type* __restrict__ b,
                                                          const int* __restrict__ adapter, const float* __restrict__ scale, const int* __restrict__ rank,
-                                                         const int* __restrict__ plan, int slots, int T, int N, int S, int R, int parts, int columns) {
+                                                         const int* __restrict__ plan, int slots, int T, int N, int S, int R, int parts, int columns,
+                                                         const typename El<P>::type* __restrict__ x0, const typename El<P>::type* __restrict__ a, int K) {
   typedef typename El<P>::type E;
+  constexpr bool BOTH = RF > 0;
+  constexpr int UR = 16 * RF + 4;
+  __shared__ __attribute__((aligned(16))) char stage[BOTH ? Down<P, BOTH ? RF : 1, 1, BOTH ? KB : 512>::ROOM : 16];
+  __shared__ __attribute__((aligned(16))) float own_u[BOTH ? 16 : 1][UR];
   constexpr int NT = Terms<P>::N, CS = TF == 1 ? 256 : RC == 4 ? 64 : 128, LD = CS + 4, HF = CS / 64, NB = 16 * TF * CS / 1024, PER_ROW = CS / 4, ROWS = 256 / PER_ROW;
   __shared__ int rows[16 * TF], waves[5];
   __shared__ __attribute__((aligned(16))) E terms[NT][RC][TF][64][8];
@@ -271,6 +286,15 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float
       }
     };
     ask(n0);
+    if constexpr (BOTH)
+      if (ra > 0) {
+        f32x4 acc[BOTH ? RF : 1];
+        down_sums<P, WHOLE, BOTH ? RF : 1, 1, BOTH ? KB : 512, 1>(acc, stage, rows, tile, ra, x0, a + (long)tile.adapter * R * K, K, 0, K);
+        if (wave == 0)
+#pragma unroll
+          for (int f = 0; f < RF; ++f) *reinterpret_cast<f32x4*>(&own_u[j][16 * f + 4 * g]) = acc[f];
+        __syncthreads();
+      }
     if (ra > 0) {
       const float sc = scale ? scale[tile.adapter] : 1.f;
       // a row's terms by four lanes (64 rows), or one of 16 rows by sixteen: lane j, g of the fragments is row j, elements 32 c + 8 g ..
@@ -281,7 +305,15 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float
         for (int c = 0; c < RC; ++c)
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
-        if (i < tile.n) {
+        if (BOTH) {
+#pragma unroll
+          for (int c = 0; c < RC; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int r = 32 * c + 8 * q + e;
+              if (r < ra && r < 16 * RF) v[c][e] = own_u[i][r];
+            }
+        } else if (i < tile.n) {
           const float* ur = u + (long)rows[i] * R;
 #pragma unroll 4
           for (int p = 0; p < parts; ++p, ur += (long)T * R)
@@ -404,11 +436,15 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float
   });
 }
 
+// Both products in one launch: A is read again for each piece of N, 64 KB of it (128 in fp32) by a workgroup at most, in 1 to 2 us, which is what a launch costs.
+// One token, bf16, 2048 x 2560, rank 8: 3.1 + 4.9 us by two launches, 6.8 by one; the whole call
+// 16.6 and 12.6.
+static bool adapter_fused(int T, int K, int R) { return T <= 64 && R <= 64 && (long)R * K <= 32768; }
 static int adapter_parts(int T, int K) { return std::max(1, std::min(T > 4096 ? 2 : T > 2048 ? 4 : 8, (K + 511) / 512)); }
 static long plan_ints(int T) { return T > WINDOW ? (long)((T + WINDOW - 1) / WINDOW) * PLAN_INTS : 0; }
 
 extern "C" long umb_seq_adapters_floats(int T, int K, int R) {
-  return T < 1 || T > (1 << 20) || K < 1 || R < 1 || R > R_MAX ? 0 : (((long)adapter_parts(T, K) * T * R + 3) & ~3L) + plan_ints(T);
+  return T < 1 || T > (1 << 20) || K < 1 || R < 1 || R > R_MAX || adapter_fused(T, K, R) ? 0 : (((long)adapter_parts(T, K) * T * R + 3) & ~3L) + plan_ints(T);
 }
 
 template <typename P, bool WHOLE, int TF>
@@ -427,6 +463,22 @@ static int adapters_launch(float* out, const float* base, const void* x, const v
     hipLaunchKernelGGL(adapter_plan_kernel, dim3(windows), dim3(64), 0, st, plan, adapter, T, S);
     UMB_LAUNCH_CHECK();
   }
+  int columns = 256;
+  while (columns < 1024 && (long)tiles * (N / (2 * columns)) >= 1024) columns *= 2;
+  const int pieces = (N + columns - 1) / columns;
+#define UP(RC, RF, KB)                                                                                                                                         \
+  if (quads) hipLaunchKernelGGL((adapter_up_kernel<P, WHOLE, true, RC, TF, RF, KB>), dim3(pieces, blocks), dim3(256), 0, st, out, base, u, (const E*)b, adapter, scale, \
+                                rank, plan, slots, T, N, S, R, parts, columns, (const E*)x, (const E*)a, K);                                                   \
+  else hipLaunchKernelGGL((adapter_up_kernel<P, WHOLE, false, RC, TF, RF, KB>), dim3(pieces, blocks), dim3(256), 0, st, out, base, u, (const E*)b, adapter, scale, \
+                          rank, plan, slots, T, N, S, R, parts, columns, (const E*)x, (const E*)a, K)
+  if constexpr (TF == 1)
+    if (adapter_fused(T, K, R)) {
+      if (R <= 16) { UP(1, 1, 1024); }
+      else if (R <= 32) { UP(1, 2, 512); }
+      else { UP(2, 4, 512); }
+      UMB_LAUNCH_CHECK();
+      return UMB_OK;
+    }
 #define DOWN(RF, KB, AHEAD)                                                                                                                                       \
   hipLaunchKernelGGL((adapter_down_kernel<P, WHOLE, RF, TF, KB, AHEAD>), dim3(parts, blocks), dim3(256), 0, st, u, (const E*)x, (const E*)a, adapter, rank, plan, slots, \
                      T, K, S, R, per)
@@ -437,17 +489,9 @@ static int adapters_launch(float* out, const float* base, const void* x, const v
   else DOWN(8, (TF == 1 && !std::is_same_v<P, F32> ? 256 : TF == 1 ? 512 : 256), 1);
 #undef DOWN
   UMB_LAUNCH_CHECK();
-  int columns = 256;
-  while (columns < 1024 && (long)tiles * (N / (2 * columns)) >= 1024) columns *= 2;
-  const int pieces = (N + columns - 1) / columns;
-#define UP(RC)                                                                                                                                             \
-  if (quads) hipLaunchKernelGGL((adapter_up_kernel<P, WHOLE, true, RC, TF>), dim3(pieces, blocks), dim3(256), 0, st, out, base, u, (const E*)b, adapter, scale, \
-                                rank, plan, slots, T, N, S, R, parts, columns);                                                                            \
-  else hipLaunchKernelGGL((adapter_up_kernel<P, WHOLE, false, RC, TF>), dim3(pieces, blocks), dim3(256), 0, st, out, base, u, (const E*)b, adapter, scale, rank, \
-                          plan, slots, T, N, S, R, parts, columns)
-  if (R <= 32) { UP(1); }
-  else if (R <= 64) { UP(2); }
-  else { UP(4); }
+  if (R <= 32) { UP(1, 0, 0); }
+  else if (R <= 64) { UP(2, 0, 0); }
+  else { UP(4, 0, 0); }
 #undef UP
   UMB_LAUNCH_CHECK();
   return UMB_OK;
@@ -455,8 +499,8 @@ static int adapters_launch(float* out, const float* base, const void* x, const v
 
 extern "C" int umb_seq_adapters(float* out, const float* base, const void* x, const void* a, const void* b, const int* adapter, const float* scale, const int* rank,
                                 int T, int N, int K, int S, int R, float* scratch, long scratch_floats, int dtype, hipStream_t st) {
-  if (!out || !base || !x || !a || !b || !adapter || !scratch || T < 1 || T > (1 << 20) || N < 1 || K < 1 || S < 1 || R < 1 || R > R_MAX || N > (1 << 24) || K > (1 << 24) ||
-      (uintptr_t)scratch % 16 || scratch_floats < umb_seq_adapters_floats(T, K, R))
+  if (!out || !base || !x || !a || !b || !adapter || T < 1 || T > (1 << 20) || N < 1 || K < 1 || S < 1 || R < 1 || R > R_MAX || N > (1 << 24) || K > (1 << 24) ||
+      (umb_seq_adapters_floats(T, K, R) > 0 && (!scratch || (uintptr_t)scratch % 16 || scratch_floats < umb_seq_adapters_floats(T, K, R))))
     return UMB_EINVAL;
   const bool quads = N % 4 == 0 && ((uintptr_t)out | (uintptr_t)base) % 16 == 0;
   const bool whole = K % 8 == 0 && R % 8 == 0 && ((uintptr_t)x | (uintptr_t)a | (uintptr_t)b) % 16 == 0;

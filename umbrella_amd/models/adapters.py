@@ -50,6 +50,6 @@ def add_adapters(base, x, a, b, adapter, scale=None, rank=None, out=None):
             raise ValueError(f"{what}: a contiguous {kind} tensor {shape} on {dev} is wanted, got {t.dtype} {tuple(t.shape)} of strides {t.stride()} on {t.device}")
     if T:
         n = _lib.load_seq().umb_seq_adapters_floats(T, K, R)
-        scratch = torch.empty(n, dtype=torch.float32, device=dev)
+        scratch = torch.empty(n, dtype=torch.float32, device=dev) if n else None
         _lib.seq_call_on(dev, "umb_seq_adapters", out, base, x, a, b, adapter, scale, rank, T, N, K, S, R, scratch, n, code)
     return out
