@@ -99,6 +99,14 @@ def test_the_table_beside_them(moves):
 
 
 @pytest.mark.gpu
+def test_a_table_shorter_than_the_moves():
+    where = torch.randperm(400, generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    table = torch.tensor([3, 399, -1, 0, 17], dtype=torch.int32)
+    got = check([(400, 1, 4, 8, torch.uint8, 1)], [(i, 200 + i, 4) for i in range(200)], table, where)
+    assert got.tolist() == [int(where[p]) if p >= 0 else -1 for p in table.tolist()]
+
+
+@pytest.mark.gpu
 def test_a_store_beyond_32_bits():
     """6 GiB: pages behind 2^32 bytes"""
     pages, page = 6144, 1 << 20

@@ -117,7 +117,7 @@ extern "C" int umb_pages_copy(const UmbPagePool* pools, int n_pools, const int* 
     const bool tab = n_table > 0 && z0 == 0;
     for (int y0 = 0; y0 < n_moves || y0 == 0; y0 += 65535) {
       const int m = n_moves - y0 < 65535 ? n_moves - y0 : 65535;
-      const long rows = tab && y0 == 0 ? std::min(256L, (n_table / (m > 0 ? m : 1) + 255) / 256) : 0;      // workgroups of the table in each row of the grid
+      const long rows = tab && y0 == 0 ? std::min(256L, n_table / (m > 0 ? m : 1) / 256 + 1) : 0;      // workgroups of the table in each row of the grid
       if (m < 1) pp.pieces = 0;                // (the table alone)
       if (pp.pieces + rows < 1) break;
       hipLaunchKernelGGL(pages_copy_kernel, dim3((unsigned)(pp.pieces + rows), m > 0 ? m : 1), dim3(256), 0, st, pp, moves + 3L * y0, m, n_pages, table, n_table, where);
