@@ -704,7 +704,7 @@ int umb_pages_copy(const UmbPagePool* pools, int n_pools, const int* moves, int 
                    umb_stream_t stream);
 
 /* Low-rank adapters of many requests beside a shared product: out[t] = base[t] + scale[a] B_a (A_a x[t]), a = adapter[t]; a outside 0 .. S - 1: base[t].
- * out and base fp32 [T][N] (may be the same); x [T][K], A [S][R][K], B [S][N][R] in `dtype`; adapter int32 [T]; scale fp32 [S] (null: 1), rank int32 [S]
+ * out and base fp32 [T][N] (may be the same; otherwise out shares no memory with what is read); x [T][K], A [S][R][K], B [S][N][R] in `dtype`; adapter int32 [T]; scale fp32 [S] (null: 1), rank int32 [S]
  * (null: R): of adapter a's R rows of A and columns of B the first rank[a] count, whatever stands in the others.  R <= 128.
  * scratch: umb_seq_adapters_floats(T, K, R) floats (no stream; 0: none, null), 16-byte aligned, anything in it; nothing is kept there between calls. */
 long umb_seq_adapters_floats(int T, int K, int R);

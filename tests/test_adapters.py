@@ -5,7 +5,7 @@ import torch
 from umbrella_amd import _lib
 from umbrella_amd.models.adapters import add_adapters, stack_adapters
 
-EINVAL, AT = -22, 1 << 20
+EINVAL, AT, OUT = -22, 1 << 20, 1 << 24
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 
@@ -236,9 +236,11 @@ def test_refusals_on_the_device():
 
 
 @pytest.mark.parametrize("kw", [dict(T=0), dict(N=0), dict(K=0), dict(S=0), dict(R=0), dict(R=129), dict(out=None), dict(base=None), dict(x=None), dict(a=None), dict(b=None),
-                                dict(adapter=None), dict(scratch=None), dict(scratch=AT + 4), dict(floats=-1), dict(dtype=3)])
+                                dict(adapter=None), dict(scratch=None), dict(scratch=AT + 4), dict(floats=-1), dict(dtype=3),
+                                # out over what is read: the base but in part, the last byte of x, a, b
+                                dict(base=OUT + 4), dict(base=OUT - 3199), dict(x=OUT), dict(x=OUT - 3199), dict(x=OUT + 3199), dict(a=OUT - 511), dict(b=OUT - 255)])
 def test_refusals_of_the_entry_point(kw):
-    a = dict(T=100, N=8, K=16, S=2, R=8, out=AT, base=AT, x=AT, a=AT, b=AT, adapter=AT, scratch=AT, floats=0, dtype=1)
+    a = dict(T=100, N=8, K=16, S=2, R=8, out=OUT, base=OUT, x=AT, a=AT, b=AT, adapter=AT, scratch=AT, floats=0, dtype=1)
     a.update(kw)
     lib = _lib.load_seq()
     n = lib.umb_seq_adapters_floats(100, 16, 8) + a["floats"]

@@ -497,10 +497,19 @@ static int adapters_launch(float* out, const float* base, const void* x, const v
   return UMB_OK;
 }
 
+static bool overlap(const void* p, long n, const void* q, long m) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  return a < b + m && b < a + n;
+}
+
 extern "C" int umb_seq_adapters(float* out, const float* base, const void* x, const void* a, const void* b, const int* adapter, const float* scale, const int* rank,
                                 int T, int N, int K, int S, int R, float* scratch, long scratch_floats, int dtype, hipStream_t st) {
   if (!out || !base || !x || !a || !b || !adapter || T < 1 || T > (1 << 20) || N < 1 || K < 1 || S < 1 || R < 1 || R > R_MAX || N > (1 << 24) || K > (1 << 24) ||
       (umb_seq_adapters_floats(T, K, R) > 0 && (!scratch || (uintptr_t)scratch % 16 || scratch_floats < umb_seq_adapters_floats(T, K, R))))
+    return UMB_EINVAL;
+  // (workgroups read x, a and b while others write; a base that is out itself is read by who writes there)
+  const long bytes = 4L * T * N, es = (long)seq_elem_bytes(dtype);
+  if (overlap(out, bytes, x, es * T * K) || overlap(out, bytes, a, es * S * R * K) || overlap(out, bytes, b, es * S * R * N) || (out != base && overlap(out, bytes, base, bytes)))
     return UMB_EINVAL;
   const bool quads = N % 4 == 0 && ((uintptr_t)out | (uintptr_t)base) % 16 == 0;
   const bool whole = K % 8 == 0 && R % 8 == 0 && ((uintptr_t)x | (uintptr_t)a | (uintptr_t)b) % 16 == 0;

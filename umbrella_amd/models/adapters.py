@@ -5,7 +5,7 @@ import torch
 
 from .. import _lib
 
-MAX_RANK = 128
+MAX_RANK, MAX_ROWS, MAX_WIDTH = 128, 1 << 20, 1 << 24
 
 
 def stack_adapters(adapters, device=None, dtype=None):
@@ -31,7 +31,7 @@ def stack_adapters(adapters, device=None, dtype=None):
 def add_adapters(base, x, a, b, adapter, scale=None, rank=None, out=None):
     """``out[t] = base[t] + scale[i] b[i] (a[i] x[t])`` with ``i = adapter[t]``; rows whose number is none of the adapters' (-1) are their base.
 
-    base, out: fp32 ``[T, N]`` (out may be base; None: a new tensor); x ``[T, K]``, a ``[S, R, K]``, b ``[S, N, R]`` of one type (bf16, fp16, fp32);
+    base, out: fp32 ``[T, N]`` (out may be base, and shares no memory with the others; None: a new tensor); x ``[T, K]``, a ``[S, R, K]``, b ``[S, N, R]`` of one type (bf16, fp16, fp32);
     adapter int32 ``[T]``; scale fp32 ``[S]``; rank int32 ``[S]``: how many of an adapter's R rows count (None: all).  All contiguous, on one GPU.
     """
     if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
@@ -40,6 +40,8 @@ def add_adapters(base, x, a, b, adapter, scale=None, rank=None, out=None):
     code = _lib.seq_dtype_code(dt)
     if dev.type != "cuda":
         raise ValueError(f"tensors on a GPU are wanted, got {dev}")
+    if T > MAX_ROWS or max(N, K) > MAX_WIDTH:
+        raise ValueError(f"up to {MAX_ROWS} rows of {MAX_WIDTH} values are possible, got x {tuple(x.shape)} and {N} columns")
     if S < 1 or not 1 <= R <= MAX_RANK or K < 1 or N < 1:
         raise ValueError(f"at least one adapter of a rank of 1 to {MAX_RANK} is wanted, got a of {tuple(a.shape)}")
     if out is None:
