@@ -254,8 +254,13 @@ def test_the_engine_admits_what_fits_and_refuses_the_rest():
         e.submit([1], 5, adapter=0)
     with pytest.raises(ValueError):
         e.generate_batch([[1], [2]], 3, sampling=[None])
-    api = e.generate(input_ids=[1, 2, 3], max_new_tokens=4, temperature=0.9, min_p=0.05, seed=3)
-    assert len(api["generated_tokens"]) == 4
+    api = [e.generate(input_ids=[1, 2, 3], max_new_tokens=12, temperature=1.5, topk=0, topp=1.0, min_p=0.001, seed=s)["generated_tokens"] for s in (3, 3, 4, None, None)]
+    assert all(len(t) == 12 for t in api) and api[0] == api[1] and len(set(map(tuple, api))) == 4        # a seed's draws are the same whatever the request's number
+    for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(top_p=1.5), dict(top_p=float("nan")), dict(min_p=-0.1), dict(min_p=2.0),
+                dict(top_k=-1), dict(top_k=1 << 31)):
+        with pytest.raises(ValueError):
+            e.submit([1], 5, sampling=Sampling(**bad))
+    assert not e.queue
     with pytest.raises(ValueError):
         engine(m, repetition_penalty=1.2).submit([1], 5, sampling=Sampling())
     assert len(engine(m, repetition_penalty=1.2, temperature=0.8).generate_batch([[1, 2]], 4, n=2)[0][1]) == 4

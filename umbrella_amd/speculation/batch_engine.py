@@ -33,7 +33,7 @@ from ..logging_config import setup_logger
 from ..models import AutoModelLM
 from ..utils import TextColors
 from .base import BaseEngine
-from .sampling import sample_rows
+from .sampling import MAX_VOCAB, sample_rows
 from .speculation_utils import IdTokenizer, is_sentence_complete_regex
 
 logger = setup_logger()
@@ -41,12 +41,17 @@ logger = setup_logger()
 
 @dataclass
 class Sampling:
-    """a request's own settings; a temperature of 0 is greedy, top_k 0 keeps all (include/umbrella_seq.h, umb_sample_requests)"""
+    """a request's own settings; a temperature of 0 is greedy, top_k 0 keeps all (include/umbrella_seq.h, umb_sample_requests).  Requests of one
+    seed draw from the same random numbers (continuation i of one from the i-th row of them); None: each has its own."""
     temperature: float = 1.0
     top_k: int = 0
     top_p: float = 1.0
     min_p: float = 0.0
-    seed: int = 0
+    seed: int | None = None
+
+    def check(self):
+        if not (0.0 <= self.temperature < float("inf") and 0.0 <= self.top_p <= 1.0 and 0.0 <= self.min_p <= 1.0 and 0 <= self.top_k < 1 << 31):
+            raise ValueError(f"a temperature of 0 and more, top_p and min_p of 0 to 1 and a top_k of 0 (all) and more are wanted, got {self}")
 
 
 @dataclass
@@ -60,6 +65,7 @@ class Request:
     recorded: int = 0                   # tokens written to the device-side history of its slot
     sampling: Sampling | None = None    # None: the engine's
     rng: random.Random | None = None
+    nth: int = 0                        # which continuation of its prompt
     adapter: int | None = None          # one of the model's
     copies: list = field(default_factory=list)       # further continuations of the same prompt
 
@@ -154,7 +160,8 @@ class BatchEngine(BaseEngine):
         mine = [r.sampling or Sampling(0.0 if self.temperature < 0.05 else self.temperature, int(self.topk), float(self.topp)) for r in reqs]
         for r in reqs:
             if r.rng is None:
-                r.rng = random.Random(f"{r.sampling.seed if r.sampling else self.seed}/{r.id}")
+                seeded = r.sampling is not None and r.sampling.seed is not None
+                r.rng = random.Random(f"{r.sampling.seed}//{r.nth}" if seeded else f"{self.seed}/{r.id}")
         host = torch.tensor([[s.temperature for s in mine], [s.top_p for s in mine], [s.min_p for s in mine], [r.rng.random() for r in reqs]], dtype=torch.float32)
         both = send(torch.cat([host.view(torch.int32), torch.tensor([[s.top_k for s in mine]], dtype=torch.int32)]), self.device)
         f = both.view(torch.float32)
@@ -209,6 +216,10 @@ class BatchEngine(BaseEngine):
             raise ValueError(f"prompt ({len(ids)}) + max_new_tokens ({max_new_tokens}) exceeds max_length {self.max_length}")
         if sampling is not None and self.repetition_penalty > 1.01:
             raise ValueError("a repetition penalty does not go with settings of a request's own")
+        if sampling is not None:
+            sampling.check()
+            if self.vocab_size > MAX_VOCAB:
+                raise ValueError(f"settings of a request's own go with up to {MAX_VOCAB} tokens, the model has {self.vocab_size}")
         if not 1 <= n <= self.max_batch:
             raise ValueError(f"1 to {self.max_batch} continuations (sequence slots) are possible, got {n}")
         if adapter is not None and not 0 <= adapter < getattr(self.target_model, "n_adapters", 0):
@@ -216,7 +227,7 @@ class BatchEngine(BaseEngine):
         if request_id is None:
             request_id, self._next_id = self._next_id, self._next_id + 1
         r = Request(request_id, ids, int(max_new_tokens), sampling=sampling, adapter=adapter)
-        r.copies = [Request((request_id, i), ids, int(max_new_tokens), sampling=sampling, adapter=adapter) for i in range(1, n)]
+        r.copies = [Request((request_id, i), ids, int(max_new_tokens), sampling=sampling, adapter=adapter, nth=i) for i in range(1, n)]
         self.queue.append(r)
         return request_id
 
@@ -406,7 +417,8 @@ class BatchEngine(BaseEngine):
         """an API request that names min_p has settings of its own; others run by the engine's"""
         if api_args.get("min_p") is None:
             return None
-        return Sampling(0.0 if self.temperature < 0.05 else float(self.temperature), int(self.topk), float(self.topp), float(api_args["min_p"]), int(api_args.get("seed", self.seed)))
+        seed = api_args.get("seed")
+        return Sampling(0.0 if self.temperature < 0.05 else float(self.temperature), int(self.topk), float(self.topp), float(api_args["min_p"]), None if seed is None else int(seed))
 
     def _request_ids(self, api_args):
         input_ids = api_args.get("input_ids", None)
