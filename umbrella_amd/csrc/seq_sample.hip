@@ -12,10 +12,12 @@
 //            further down weighs less than 2^-46 of the row).  Bins lie on one lattice, floor(32 x / T), and masses are relative to their bin's middle, so
 //            that slices' add up as whole numbers, count and mass in one 64-bit atomic
 //   collect  the row's bins, summed up from the top, say which bins hold the k-th value, the ends of top-p and min-p and the token drawn (intervals, since
-//            the mass behind p and u is known to a bin only); their tokens are collected, from slices that have any.  A row of a small k has counts alone, and
+//            the mass behind p and u is known to a bin only); their tokens are collected.  A row of a small k has counts alone, and
 //            all tokens down to the k-th value's bin are collected
 //   resolve  a row's collected tokens by one workgroup: where they are many, bins again, up to 256 in each bin; then in order: the exact ends, then the draw
-// Bound by the logits: the first launch reads them from memory, the second a part of them again, from the cache behind it.
+// us (slices, collect, resolve): a row of 32000 3.8, 8.2, 10; 8 of 128256 5.2, 13.7, 10.9; 48 of 151936 12.1, 22.8, 17.4; 256 of 128256 37.9, 33.7, 14.9.
+// Bound by the logits where rows are many: the first launch reads them from memory, the second once more, from the cache behind it; by launches and barriers where
+// they are few.
 // Rows of up to SMALL_V values are taken whole by the last launch alone.  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
 // the thousand), is searched eight bits of the key at a time, by one workgroup.
 #include "seq_common.h"
@@ -186,7 +188,7 @@ __device__ __attribute__((noinline)) void sample_slow(int r, int* __restrict__ t
 }
 
 // ------------------------------------------------------------------ bins
-constexpr int BINS = 1024, SMALL_V = 2048, CAP = 2048, K_COUNT = 1024, P_MAX = 64;
+constexpr int BINS = 1024, SMALL_V = 2048, CAP = 2048, K_COUNT = 1024, P_MAX = 64, FEW = 128;
 constexpr double PER_T = 32.0, LATTICE = 1099511627776.0;         // bins a T; beyond 2^40 neighbouring floats are 2^16 bins apart and more
 constexpr double MAGIC = 4503599627370496.0;                     // 2^52: added to a number below 2^51, it leaves the nearest whole number in the low bits
 constexpr double BIN_ONE = 4294967296.0;                         // a bin's masses, in 2^-32 of its middle's weight: 48 bits for 2^15 of them, 16 above for their number
@@ -726,7 +728,8 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       if (slot[tid] >= 0) bin_of[slot[tid]] = (short)tid;
     }
   }
-  const bool many = !SMALL && found > CAP;
+  // (putting in order takes 13 us for 1024 tokens and more, 6 for 300, 1.6 for 64 and fewer; the bins and looking again 5, and a dozen tokens are left)
+  const bool many = !SMALL && found > FEW;
   // bins of the collected tokens: all in one (front of it nothing); those of collect; or `cut` in each of those
   int cut = 1;
   if (many) while (2 * cut * slots <= CAP && cut < 256) cut *= 2;
@@ -949,9 +952,11 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   __syncthreads();
   if (how_k == 1 && got[0] == 0) { count = k; mass = masses; }
   const double limit = fmax(set.p, 0.0) * mass;
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (e0 + e < n && p_binds && in[e] >= limit) atomicMin(&got[1], e0 + e);
+  auto first_of = [&](bool x, bool y, int* to) {             // (one atomic a wave)
+    const unsigned long long one = __ballot(x || y);
+    if (one && lane == __ffsll(one) - 1) atomicMin(to, x ? e0 : e0 + 1);
+  };
+  first_of(e0 < n && p_binds && in[0] >= limit, e0 + 1 < n && p_binds && in[1] >= limit, &got[1]);
   __syncthreads();
   const int kp = got[1];
 #pragma unroll
@@ -962,9 +967,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   if (count < 1) { count = 1; mass = 1.0; }
   // the draw: the first over the goal, the last kept one where the sums' rounding leaves none
   const double goal = set.u * mass;
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (e0 + e < n && q[e] && rank[e] < count && in[e] > goal) atomicMin(&got[2], e0 + e);
+  first_of(e0 < n && q[0] && rank[0] < count && in[0] > goal, e0 + 1 < n && q[1] && rank[1] < count && in[1] > goal, &got[2]);
   __syncthreads();
   int at = got[2];
   if (at >= CAP) {
