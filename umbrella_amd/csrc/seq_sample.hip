@@ -15,7 +15,7 @@
 //            the mass behind p and u is known to a bin only); their tokens are collected.  A row of a small k has counts alone, and
 //            all tokens down to the k-th value's bin are collected
 //   resolve  a row's collected tokens by one workgroup: where they are many, bins again, up to 256 in each bin; then in order: the exact ends, then the draw
-// us (slices, collect, resolve): a row of 32000 3.8, 8.2, 10; 8 of 128256 5.2, 13.7, 10.9; 48 of 151936 12.1, 22.8, 17.4; 256 of 128256 37.9, 33.7, 14.9.
+// us (slices, collect, resolve): a row of 32000 3.8, 8.2, 10; 8 of 128256 5.2, 13.7, 10.9; 48 of 151936 12.2, 20.5, 16.8; 256 of 128256 37.5, 31, 14.2.
 // Bound by the logits where rows are many: the first launch reads them from memory, the second once more, from the cache behind it; by launches and barriers where
 // they are few.
 // Rows of up to SMALL_V values are taken whole by the last launch alone.  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
@@ -417,16 +417,13 @@ template <int NT, typename T> __device__ __forceinline__ T sum_upto(T v, T* room
   const T before = __shfl(w, wave > 0 ? wave - 1 : 0, 64);
   return wave > 0 ? v + before : v;
 }
-// how many threads of NT hold a, and how many b; `room` [NT / 64] is this call's alone
+// how many threads hold a, and how many b; `cell`, 0, is this call's alone (one addition a wave: sixteen waves that read sixteen words each took 1 us and more)
 struct Two { int a, b; };
-template <int NT> __device__ __forceinline__ Two how_many(bool a, bool b, int* room) {
-  const int lane = threadIdx.x & 63;
-  const int n = __popcll(__ballot(a)) | (__popcll(__ballot(b)) << 16);
-  if (lane == 0) room[threadIdx.x >> 6] = n;
+__device__ __forceinline__ Two how_many(bool a, bool b, int* cell, bool also_a = false, bool also_b = false) {
+  const int n = (__popcll(__ballot(a)) + __popcll(__ballot(also_a))) | ((__popcll(__ballot(b)) + __popcll(__ballot(also_b))) << 16);
+  if ((threadIdx.x & 63) == 0 && n) atomicAdd(cell, n);
   __syncthreads();
-  int w = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 64; ++i) w += room[i];
+  const int w = *cell;
   return Two{w & 0xffff, w >> 16};
 }
 
@@ -437,7 +434,7 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
                                                               const float* __restrict__ top_p, const float* __restrict__ min_p) {
   constexpr int NT = BINS;
   __shared__ double m_in[BINS], wave_m[NT / 64];
-  __shared__ int shift[P_MAX], c_in[BINS], wave_c[NT / 64], rooms[3][NT / 64], found;
+  __shared__ int shift[P_MAX], c_in[BINS], wave_c[NT / 64], cells[3], found;
   __shared__ float bounds[4][2];
   const int r = blockIdx.y, P = cut.P, b = threadIdx.x, lane = b & 63;
   int p = blockIdx.x;                        // chunk
@@ -454,6 +451,7 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
     shift[b] = d < BINS && counts(head, top, per) ? (int)d : BINS;
   }
   if (b == 0) found = 0;
+  if (b < 3) cells[b] = 0;
   __syncthreads();
   unsigned long long q = 0ull;
   int c = 0;
@@ -480,7 +478,7 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
   // the bins that each end may lie in: k0, [p0, p1], [m0, m1], [d0, d1]; BINS: nowhere
   const int k = set.m > 1.0 ? 1 : set.k;
   const bool whole = top_k && top_k[r] >= 1 && top_k[r] <= K_COUNT, k_binds = k < c_all;
-  const int k0 = k_binds ? how_many<NT>(c < k, false, rooms[0]).a : BINS;
+  const int k0 = k_binds ? how_many(c < k, false, &cells[0]).a : BINS;
   const bool k_exact = k_binds && c_in[k0] == k;
   bool p_binds = false, m_binds = false;
   int m0 = BINS, m1 = BINS, from[4] = {0, BINS, BINS, BINS}, to[4] = {min(k0, BINS - 1), -1, -1, -1};       // runs of bins that are wanted
@@ -488,7 +486,7 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
     const double mk_hi = k_binds ? m_in[k0] : all, mk_lo = !k_binds || k_exact ? mk_hi : k0 > 0 ? m_in[k0 - 1] : 0.0;
     int p0 = BINS, p1 = BINS;
     if (set.p < 1.0) {
-      const Two n = how_many<NT>(m < set.p * mk_lo - slack, m_ex < set.p * mk_hi + slack, rooms[1]);
+      const Two n = how_many(m < set.p * mk_lo - slack, m_ex < set.p * mk_hi + slack, &cells[1]);
       p0 = n.a;
       p1 = max(0, n.b - 1);
     }
@@ -505,7 +503,7 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
     if (p_binds) { lo = fmin(lo, set.p * mk_lo - slack); hi = fmin(hi, m_in[min(p1, BINS - 1)]); }
     if (m_binds) { lo = fmin(lo, m0 > 0 ? m_in[m0 - 1] : 0.0); hi = fmin(hi, m_in[m1]); }
     lo = fmax(lo, 0.0);
-    const Two d = how_many<NT>(m <= set.u * lo - slack, m_ex <= set.u * hi + slack, rooms[2]);
+    const Two d = how_many(m <= set.u * lo - slack, m_ex <= set.u * hi + slack, &cells[2]);
     const int d0 = d.a, d1 = d.b - 1;
     from[0] = d0;
     to[0] = min(d1, end);
@@ -650,7 +648,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   __shared__ double front_m[CAP];                                  // mass and count in front of each bin
   __shared__ int front_c[CAP], start[CAP];                         // where a bin's tokens start in v
   __shared__ u64 wide[ST / 64];
-  __shared__ int narrow[ST / 64], rooms[6][ST / 64];
+  __shared__ int narrow[ST / 64], cells[3];
   __shared__ short slot[BINS], bin_of[BINS];
   __shared__ unsigned char want[CAP];
   __shared__ SlowRoom room;
@@ -757,6 +755,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     }
   };
   if (tid < 4) got[tid] = CAP;
+  if (tid < 3) cells[tid] = 0;
   if (tid == 0) { taken = 0; sum_c = 0; sum_m = 0ull; }
   if (many) for (int i = tid; i < CAP; i += ST) { raw[i] = 0ull; start[i] = 0; }
   __syncthreads();
@@ -850,8 +849,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     }
     const double slack = slack_of * mass;
     auto before = [&](bool a0, bool a1, bool b0, bool b1, int call) -> Two {       // bins, of both a thread's
-      const Two x = how_many<ST>(is[0] && a0, is[0] && b0, rooms[2 * call]), y = how_many<ST>(is[1] && a1, is[1] && b1, rooms[2 * call + 1]);
-      return Two{x.a + y.a, x.b + y.b};
+      return how_many(is[0] && a0, is[0] && b0, &cells[call], is[1] && a1, is[1] && b1);
     };
     const int k0 = how_k == 1 ? before(c_in[0] < k, c_in[1] < k, false, false, 0).a : used;
     double lo = mass, hi = mass;
