@@ -15,7 +15,7 @@
 //            the mass behind p and u is known to a bin only); their tokens are collected.  A row of a small k has counts alone, and
 //            all tokens down to the k-th value's bin are collected
 //   resolve  a row's collected tokens by one workgroup: where they are many, bins again, up to 256 in each bin; then in order: the exact ends, then the draw
-// us (slices, collect, resolve): a row of 32000 3.8, 8.2, 10; 8 of 128256 5.2, 13.7, 10.9; 48 of 151936 12.2, 20.5, 16.8; 256 of 128256 37.5, 31, 14.2.
+// us (slices, collect, resolve): a row of 32000 3.8, 7.9, 10; 8 of 128256 5.2, 12.2, 10.9; 48 of 151936 12.2, 19.6, 16.8; 256 of 128256 37.5, 29.5, 14.2.
 // Bound by the logits where rows are many: the first launch reads them from memory, the second once more, from the cache behind it; by launches and barriers where
 // they are few.
 // Rows of up to SMALL_V values are taken whole by the last launch alone.  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
@@ -417,6 +417,26 @@ template <int NT, typename T> __device__ __forceinline__ T sum_upto(T v, T* room
   const T before = __shfl(w, wave > 0 ? wave - 1 : 0, 64);
   return wave > 0 ? v + before : v;
 }
+// two sums at once, in rooms that nobody holds yet
+template <int NT, typename T, typename U> __device__ __forceinline__ void sums_upto(T& v, U& w, T* room_v, U* room_w) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  v = wave_upto(v);
+  w = wave_upto(w);
+  if (lane == 63) { room_v[wave] = v; room_w[wave] = w; }
+  __syncthreads();
+  T a = lane < wave ? room_v[lane] : T(0);   // (of the waves in front, of which there are 15 at most)
+  U b = lane < wave ? room_w[lane] : U(0);
+  auto row = [](auto& x) {
+    x += lanes<0x111, 0xf>(x);
+    x += lanes<0x112, 0xf>(x);
+    x += lanes<0x114, 0xf>(x);
+    x += lanes<0x118, 0xf>(x);
+  };
+  row(a);
+  row(b);
+  v += __shfl(a, 15, 64);
+  w += __shfl(b, 15, 64);
+}
 // how many threads hold a, and how many b; `cell`, 0, is this call's alone (one addition a wave: sixteen waves that read sixteen words each took 1 us and more)
 struct Two { int a, b; };
 __device__ __forceinline__ Two how_many(bool a, bool b, int* cell, bool also_a = false, bool also_b = false) {
@@ -455,21 +475,25 @@ __global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restric
   __syncthreads();
   unsigned long long q = 0ull;
   int c = 0;
-#pragma unroll 8
-  for (int i = 0; i < P; ++i) {
-    const int k = b - shift[i];
-    const unsigned long long v = s.bins[i * BINS + max(k, 0)];
-    if (k >= 0) {
-      c += (int)(v >> 48);
-      q += v & 0xffffffffffffull;
+  constexpr int BATCH = NE <= 8 ? 16 : 8;    // slices asked for together
+  for (int i0 = 0; i0 < P; i0 += BATCH) {
+    unsigned long long v[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int k = i0 + i < P ? b - shift[i0 + i] : -1;
+      v[i] = k >= 0 ? s.bins[(i0 + i) * BINS + k] : 0ull;
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      c += (int)(v[i] >> 48);
+      q += v[i] & 0xffffffffffffull;
     }
   }
   // a bin's middle beside the largest; beside an infinite one, or one beyond the lattice, only its equals count
   const bool flat = top == INFINITY || !(fabs((double)top * per) < LATTICE);
   double m = flat ? (b == 0 ? (double)c : 0.0) : (double)q * (1.0 / BIN_ONE) * exp_down((first - b + 0.5 - line) * (1.0 / PER_T));
   const int c_own = c;
-  c = sum_upto<NT>(c, wave_c);
-  m = sum_upto<NT>(m, wave_m);
+  sums_upto<NT>(c, m, wave_c, wave_m);
   c_in[b] = c;
   m_in[b] = m;
   __syncthreads();
@@ -813,8 +837,10 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     const int b0 = 2 * tid;
     const u64 q0 = raw[b0], q1 = raw[b0 + 1];
     const int c0 = start[b0], c1 = start[b0 + 1];
-    const u64 qs = sum_upto<ST>(q0 + q1, wide);
-    const int cs = sum_upto<ST>(c0 + c1, narrow);
+    u64 qs = q0 + q1;
+    int cs = c0 + c1;
+    __syncthreads();
+    sums_upto<ST>(qs, cs, wide, narrow);
     __syncthreads();
     raw[b0] = qs - q0 - q1;
     raw[b0 + 1] = qs - q1;
