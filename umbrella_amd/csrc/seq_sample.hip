@@ -15,7 +15,7 @@
 //            the mass behind p and u is known to a bin only); their tokens are collected.  A row of a small k has counts alone, and
 //            all tokens down to the k-th value's bin are collected
 //   resolve  a row's collected tokens by one workgroup: where they are many, bins again, up to 256 in each bin; then in order: the exact ends, then the draw
-// us (slices, collect, resolve): a row of 32000 3.8, 7.9, 10; 8 of 128256 5.2, 12.2, 10.9; 48 of 151936 12.2, 19.6, 16.8; 256 of 128256 37.5, 29.5, 14.2.
+// us (slices, collect, resolve): a row of 32000 3.8, 8, 9.9; 8 of 128256 5.2, 11.3, 10.2; 48 of 151936 12.2, 19.6, 16.6; 256 of 128256 37.4, 29.4, 14.
 // Bound by the logits where rows are many: the first launch reads them from memory, the second once more, from the cache behind it; by launches and barriers where
 // they are few.
 // Rows of up to SMALL_V values are taken whole by the last launch alone.  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
@@ -673,7 +673,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   __shared__ int front_c[CAP], start[CAP];                         // where a bin's tokens start in v
   __shared__ u64 wide[ST / 64];
   __shared__ int narrow[ST / 64], cells[3];
-  __shared__ short slot[BINS], bin_of[BINS];
+  __shared__ short slot[BINS];
   __shared__ unsigned char want[CAP];
   __shared__ SlowRoom room;
   __shared__ int from[P_MAX + 1], got[4], ranks, taken, sum_c;
@@ -686,7 +686,14 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   float top = -INFINITY;
   int first_at = 0, had = 0;
   RowSaid said{};
-  if constexpr (!SMALL) said = s.sums->said;     // (asked for with the heads; a greedy row has none)
+  double bin_m = 0.0;                        // of bin tid
+  int bin_c = 0, bin_slot = -1;
+  if constexpr (!SMALL) {                    // (asked for with the heads; of a greedy row it is whatever stands there)
+    said = s.sums->said;
+    bin_m = s.sums->mass[tid];
+    bin_c = s.sums->count[tid];
+    bin_slot = s.sums->slot[tid];
+  }
   if constexpr (SMALL) {
     u64 best = 0ull;
     for (int i = tid; i < V; i += ST) {
@@ -724,6 +731,9 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   bool whole = true, p_binds = set.p < 1.0, m_binds = set.m > 0.0 && set.m <= 1.0;
   const int k = set.m > 1.0 ? 1 : set.k;
   int m0 = 0, m1 = BINS - 1, found = 0;
+  static_assert(CAP * 8 >= BINS * 12 && BINS == ST);
+  double* const slot_m = reinterpret_cast<double*>(v);               // mass and count in front of each collected bin, while v holds no tokens
+  int* const slot_c = reinterpret_cast<int*>(v + BINS);
   if constexpr (!SMALL) {
     if (__ballot(had > row_cut.cap)) {
       sample_slow(r, tokens, probs, row, V, set, top, room);
@@ -745,9 +755,10 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       m1 = said.m1;
     }
     slots = said.slots;
-    if (tid < BINS) {
-      slot[tid] = s.sums->slot[tid];
-      if (slot[tid] >= 0) bin_of[slot[tid]] = (short)tid;
+    slot[tid] = (short)bin_slot;
+    if (found > FEW && bin_slot >= 0) {
+      slot_m[bin_slot] = bin_m;
+      slot_c[bin_slot] = bin_c;
     }
   }
   // (putting in order takes 13 us for 1024 tokens and more, 6 for 300, 1.6 for 64 and fewer; the bins and looking again 5, and a dozen tokens are left)
@@ -858,11 +869,11 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       ex[e] = in[e] = 0.0;
       c_ex[e] = c_in[e] = 0;
       if (is[e]) {
-        const int z = b / cut * cut, j = bin_of[b / cut];
+        const int z = b / cut * cut, j = b / cut;
         const u64 q = raw[b] - (whole ? 0ull : raw[z]);
-        ex[e] = (whole ? 0.0 : s.sums->mass[j]) + (double)q * (1.0 / FINE_ONE);
-        in[e] = (whole ? 0.0 : s.sums->mass[j]) + (double)(q + (e ? q1 : q0)) * (1.0 / FINE_ONE);
-        c_ex[e] = whole ? start[b] : s.sums->count[j] + start[b] - start[z];
+        ex[e] = (whole ? 0.0 : slot_m[j]) + (double)q * (1.0 / FINE_ONE);
+        in[e] = (whole ? 0.0 : slot_m[j]) + (double)(q + (e ? q1 : q0)) * (1.0 / FINE_ONE);
+        c_ex[e] = whole ? start[b] : slot_c[j] + start[b] - start[z];
         c_in[e] = c_ex[e] + (e ? c1 : c0);
       }
       front_m[b] = ex[e];
@@ -932,7 +943,8 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       return;
     }
   } else if (!SMALL && !whole) {
-    if (tid < BINS) { front_m[tid] = s.sums->mass[tid]; front_c[tid] = s.sums->count[tid]; }
+    front_m[tid] = bin_m;
+    front_c[tid] = bin_c;
   } else if (tid == 0) { front_m[0] = 0.0; front_c[0] = 0; }
   int size = 64;
   while (size < n) size <<= 1;
