@@ -9,7 +9,8 @@
 //
 // Bound by memory: x, A, B and the base are read once and out is written once, in pieces of 256 contiguous bytes and more, which fragments read from
 // memory directly (16 rows x 64 bytes) are not: they took 46 + 71 us where
-// staging takes 9.6 + 15.8 (1999 tokens, fp16, 4096 x 4096, rank 32; 8192 tokens, bf16, 4096 x 6144, rank 64: 83 + 222, 30 + 99).
+// staging takes 8.5 + 15.5 (1999 tokens, fp16, 4096 x 4096, rank 32; 8192 tokens, bf16, 4096 x 6144, rank 64: 83 + 222, 31 + 92).  Of those 31 loads are
+// 11, the products 5; the rest is LDS and its barriers, which more or deeper stages (28 - 33) do not change.
 //
 // u enters the second product with 22 bits or more: three bf16 terms (each the rest that the one before left), two fp16 ones behind a power of two per row
 // (whatever u's size), or itself in fp32.
@@ -123,16 +124,25 @@ __device__ __forceinline__ Tile tile_of_plan(const int* __restrict__ p, int k, i
   return Tile{p[1 + k], n};
 }
 
+// Which block of the grid this one is.  Blocks go round the eight dies; with a plan each die takes neighbours, whose adapters its cache then holds
+// (the second product of 8192 rows, 4096 x 6144, rank 64: 99 -> 92 us).
+struct Place { int x, y; };
+template <int TF> __device__ __forceinline__ Place place_of() {
+  if constexpr (TF == 1) return Place{(int)blockIdx.x, (int)blockIdx.y};
+  const unsigned all = gridDim.x * gridDim.y, l = blockIdx.y * gridDim.x + blockIdx.x, die = l % 8, at = die * (all / 8) + min(die, all % 8) + l / 8;
+  return Place{(int)(at % gridDim.x), (int)(at / gridDim.x)};
+}
+
 // each tile that is this block's: block = row, or, with a plan (TF 4), every slots-th tile of a window
 template <int TF, typename F>
-__device__ __forceinline__ void each_tile(const int* plan, int slots, int T, int S, const int* adapter, int* rows, int* waves, F f) {
+__device__ __forceinline__ void each_tile(int block, const int* plan, int slots, int T, int S, const int* adapter, int* rows, int* waves, F f) {
   if constexpr (TF == 1) {
-    const Tile t = tile_of_row<16>(blockIdx.y, T, S, adapter, rows, waves);
+    const Tile t = tile_of_row<16>(block, T, S, adapter, rows, waves);
     if (t.n > 0) f(t);
   } else {
-    const int* p = plan + (long)(blockIdx.y / slots) * PLAN_INTS;
+    const int* p = plan + (long)(block / slots) * PLAN_INTS;
     const int n = p[0];
-    for (int k = blockIdx.y % slots; k < n; k += slots) f(tile_of_plan(p, k, rows));
+    for (int k = block % slots; k < n; k += slots) f(tile_of_plan(p, k, rows));
   }
 }
 
@@ -213,8 +223,9 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u
   __shared__ int rows[16 * TF], waves[5];
   __shared__ __attribute__((aligned(16))) char stage[Down<P, RF, TF, KB>::ROOM];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int k0 = blockIdx.x * per, k1 = min(K, k0 + per);
-  each_tile<TF>(plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
+  const Place at = place_of<TF>();
+  const int k0 = at.x * per, k1 = min(K, k0 + per);
+  each_tile<TF>(at.y, plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
     if (tile.adapter < 0) return;
     const int ra = rank ? min(max(rank[tile.adapter], 0), R) : R;
     if (ra < 1) return;
@@ -222,7 +233,7 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u
     down_sums<P, WHOLE, RF, TF, KB, AHEAD>(acc, stage, rows, tile, ra, x, a + (long)tile.adapter * R * K, K, k0, k1);
     const int own = TF == 4 ? wave * 16 + j : j;
     if ((TF == 1 && wave > 0) || own >= tile.n) return;
-    float* to = u + ((long)blockIdx.x * T + rows[own]) * R;
+    float* to = u + ((long)at.x * T + rows[own]) * R;
 #pragma unroll
     for (int f = 0; f < RF; ++f) {
       const int r = 16 * f + 4 * g;
@@ -258,8 +269,9 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float
   __shared__ float power[16 * TF];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const int row = threadIdx.x / PER_ROW, quad = threadIdx.x % PER_ROW;
-  const int n0 = blockIdx.x * columns, n1 = min(N, n0 + columns);
-  each_tile<TF>(plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
+  const Place at = place_of<TF>();
+  const int n0 = at.x * columns, n1 = min(N, n0 + columns);
+  each_tile<TF>(at.y, plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
     const int ra = tile.adapter < 0 ? 0 : rank ? min(max(rank[tile.adapter], 0), R) : R;
     if (ra < 1 && out == base) return;
     f32x4 x[NB];
