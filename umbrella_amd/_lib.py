@@ -445,7 +445,8 @@ def _stream_of(index: int) -> int:
 def seq_call(name: str, *args):
     """call an entry point of libumbrella_seq.so on the current stream (tensors -> pointers, structs by reference)"""
     lib = _seq_lib or load_seq()
-    conv = [a.data_ptr() if isinstance(a, torch.Tensor) else C.byref(a) if isinstance(a, C.Structure) else a for a in args]
+    # (plain numbers first: isinstance of a tensor is a call of its own for whatever is none)
+    conv = [a if a is None or type(a) is int else a.data_ptr() if isinstance(a, torch.Tensor) else C.byref(a) if isinstance(a, C.Structure) else a for a in args]
     rc = getattr(lib, name)(*conv, _stream_of(torch.cuda.current_device()))
     if rc != 0:
         raise UmbError(f"libumbrella_seq {name} failed with code {rc}")
