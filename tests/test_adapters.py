@@ -209,6 +209,18 @@ def test_captured_and_on_streams():
         assert torch.equal(got, beside)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("T", [257, 512, 700])
+def test_as_many_adapters_as_rows(name, T):
+    """every row of a window its own, in any order; the same bits again"""
+    kw = make(T, 40, 36, 900, 8, TYPES[name], seed=T, ids="any", ranks=[8, 3, 0, 5])
+    kw["adapter"] = torch.randperm(900, generator=torch.Generator().manual_seed(T))[:T].to(torch.int32)
+    assert torch.equal(check(kw), check(kw))
+    kw["adapter"][::3] = torch.tensor([-1, 1 << 30, -(1 << 31), 900])[torch.arange(len(kw["adapter"][::3])) % 4].to(torch.int32)
+    check(kw)
+
+
 def test_refusals_of_the_wrapper():
     kw = make(4, 16, 8, 2, 8, torch.float32)
     kw.pop("rank")

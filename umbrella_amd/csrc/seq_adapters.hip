@@ -5,12 +5,12 @@
 //
 // Two launches (one where the factors are small): u = A x, fp32, summed over K in `parts` pieces; then out.  Rows of one adapter are taken together, so that A and B are read once for them.
 // Up to 256 rows: tiles of 16; the row whose place among its adapter's rows is a multiple of 16 stands for those from it on, and every other row's block is
-// empty: nothing is sorted or counted beforehand.  More rows: tiles of 64, and a launch in front works them out once for each window of 256.
+// empty: nothing is sorted or counted beforehand.  More rows: tiles of 64, worked out for each window of 256.
 //
 // Bound by memory: x, A, B and the base are read once and out is written once, in pieces of 256 contiguous bytes and more, which fragments read from
 // memory directly (16 rows x 64 bytes) are not: they took 46 + 71 us where
-// staging takes 8.5 + 15.5 (1999 tokens, fp16, 4096 x 4096, rank 32; 8192 tokens, bf16, 4096 x 6144, rank 64: 83 + 222, 31 + 92).  Of those 31 loads are
-// 11, the products 5; the rest is LDS and its barriers, which more or deeper stages (28 - 33) do not change.
+// staging takes 11.7 + 14.8 (1999 tokens, fp16, 4096 x 4096, rank 32; 8192 tokens, bf16, 4096 x 6144, rank 64: 83 + 222, 34 + 93).  Of those 34 the plan is 3,
+// loads are 11, the products 5; the rest is LDS and its barriers, which more or deeper stages (28 - 33 for 31) did not change.
 //
 // u enters the second product with 22 bits or more: three bf16 terms (each the rest that the one before left), two fp16 ones behind a power of two per row
 // (whatever u's size), or itself in fp32.
@@ -72,49 +72,70 @@ template <int TILE> __device__ __forceinline__ Tile tile_of_row(int t, int T, in
 }
 
 // More rows: plan, of each window: how many tiles; their adapters; their first places and sizes (first + 1024 n); the window's rows, those of a tile side by
-// side.  A wave a window, four rows a lane: adapter by adapter, in the order of their first rows, whose rows are found by comparisons and placed by counting
-// bits.  (All rows against all by 1024 threads took 7.6 us whatever there was; this 4 where a window has a few adapters.)
-constexpr int PLAN_TILE = 64, PLAN_INTS = 1 + 3 * WINDOW;
-__global__ __launch_bounds__(64) void adapter_plan_kernel(int* __restrict__ plan, const int* __restrict__ adapter, int T, int S) {
-  constexpr int NE = WINDOW / 64;
-  const int lane = threadIdx.x, t0 = blockIdx.x * WINDOW;
-  int* p = plan + (long)blockIdx.x * PLAN_INTS;
-  int id[NE];
-  unsigned long long left[NE];
+// side.  An adapter is known by its first row, which a table of 512 places finds whatever the adapters' numbers are; a row's place among its adapter's is counted
+// in its wave and over the waves in front, so that every workgroup that makes a window's plan makes the same.  Every one of the first product does, and one leaves it
+// for the second (in a launch in front, adapter by adapter: 26.8 us where this takes 24.8 for 1999 rows of 4 adapters; 300 rows of 64 in any order 40 against 20).
+constexpr int PLAN_TILE = 64, PLAN_INTS = 1 + 3 * WINDOW, PLACES = 2 * WINDOW;
+struct PlanRoom { int key[PLACES], first[PLACES], count[WINDOW / 64][WINDOW], front[WINDOW], sums[WINDOW / 64]; };
+__device__ __forceinline__ void plan_window(int* p, PlanRoom& room, int window, const int* __restrict__ adapter, int T, int S) {
+  constexpr int WAVES = WINDOW / 64;
+  const int i = threadIdx.x, lane = i & 63, wave = i >> 6, t = window * WINDOW + i;
+  const bool is = t < T;
+  int id = is ? adapter[t] : -1;
+  if (id < 0 || id >= S) id = -1;
+  for (int k = i; k < PLACES; k += WINDOW) { room.key[k] = -2; room.first[k] = WINDOW; }
 #pragma unroll
-  for (int e = 0; e < NE; ++e) {
-    const int t = t0 + 64 * e + lane;
-    id[e] = t < T ? adapter[t] : -2;
-    if (t < T && (id[e] < 0 || id[e] >= S)) id[e] = -1;
-  }
-#pragma unroll
-  for (int e = 0; e < NE; ++e) left[e] = __ballot(id[e] != -2);
-  const unsigned long long below = (1ull << lane) - 1ull;
-  int tiles = 0, front = 0;
-  for (;;) {
-    int mine = -2;
-#pragma unroll
-    for (int e = NE - 1; e >= 0; --e)
-      if (left[e]) mine = __builtin_amdgcn_readlane(id[e], __ffsll(left[e]) - 1);
-    if (mine == -2) break;
-    int n = 0;
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      const bool same = id[e] == mine;
-      const unsigned long long bal = __ballot(same);
-      if (same) p[1 + 2 * WINDOW + front + n + __popcll(bal & below)] = t0 + 64 * e + lane;
-      n += __popcll(bal);
-      left[e] &= ~bal;
+  for (int w = 0; w < WAVES; ++w) room.count[w][i] = 0;
+  __syncthreads();
+  int at = (int)(((unsigned)id * 2654435761u) >> 23);        // 0 .. 511
+  if (is) {
+    // (256 keys at most in 512 places: each finds its own or a free one)
+    for (;;) {
+      const int was = atomicCAS(&room.key[at], -2, id);
+      if (was == -2 || was == id) break;
+      at = (at + 1) % PLACES;
     }
-    const int k = (n + PLAN_TILE - 1) / PLAN_TILE;
-    if (lane < k) {
-      p[1 + tiles + lane] = mine;
-      p[1 + WINDOW + tiles + lane] = front + lane * PLAN_TILE + 1024 * min(PLAN_TILE, n - lane * PLAN_TILE);
-    }
-    tiles += k;
-    front += n;
+    atomicMin(&room.first[at], i);
   }
-  if (lane == 0) p[0] = tiles;
+  __syncthreads();
+  const int own = is ? room.first[at] : WINDOW;
+  unsigned long long same = __ballot(own == __builtin_amdgcn_readfirstlane(own));
+  if (same != ~0ull) {
+    unsigned lo = 0u, hi = 0u;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      lo |= own == __builtin_amdgcn_readlane(own, k) ? 1u << k : 0u;
+      hi |= own == __builtin_amdgcn_readlane(own, 32 + k) ? 1u << k : 0u;
+    }
+    same = lo | (unsigned long long)hi << 32;
+  }
+  int place = __popcll(same & ((1ull << lane) - 1ull));
+  if (is && place == 0) room.count[wave][own] = __popcll(same);
+  __syncthreads();
+  if (is)
+    for (int w = 0; w < wave; ++w) place += room.count[w][own];
+  // of the adapter whose first row is row i
+  int n = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) n += room.count[w][i];
+  const int k = (n + PLAN_TILE - 1) / PLAN_TILE;
+  int upto = n | k << 16;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(upto, o, 64); if (lane >= o) upto += v; }
+  if (lane == 63) room.sums[wave] = upto;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) { if (w < wave) upto += room.sums[w]; all += room.sums[w]; }
+  const int front = (upto & 0xffff) - n, tile = (upto >> 16) - k;
+  room.front[i] = front;
+  for (int e = 0; e < k; ++e) {
+    p[1 + tile + e] = id;
+    p[1 + WINDOW + tile + e] = front + e * PLAN_TILE + 1024 * min(PLAN_TILE, n - e * PLAN_TILE);
+  }
+  if (i == 0) p[0] = all >> 16;
+  __syncthreads();
+  if (is) p[1 + 2 * WINDOW + room.front[own] + place] = t;
 }
 __device__ __forceinline__ Tile tile_of_plan(const int* __restrict__ p, int k, int* rows) {
   const int said = p[1 + WINDOW + k], n = said / 1024, first = said % 1024;
@@ -135,13 +156,12 @@ template <int TF> __device__ __forceinline__ Place place_of() {
 
 // each tile that is this block's: block = row, or, with a plan (TF 4), every slots-th tile of a window
 template <int TF, typename F>
-__device__ __forceinline__ void each_tile(int block, const int* plan, int slots, int T, int S, const int* adapter, int* rows, int* waves, F f) {
+__device__ __forceinline__ void each_tile(int block, const int* p, int slots, int T, int S, const int* adapter, int* rows, int* waves, F f) {
   if constexpr (TF == 1) {
     const Tile t = tile_of_row<16>(block, T, S, adapter, rows, waves);
     if (t.n > 0) f(t);
   } else {
-    const int* p = plan + (long)(block / slots) * PLAN_INTS;
-    const int n = p[0];
+    const int n = p[0];                      // p: its window's plan
     for (int k = block % slots; k < n; k += slots) f(tile_of_plan(p, k, rows));
   }
 }
@@ -218,14 +238,22 @@ __device__ __forceinline__ void down_sums(f32x4 (&acc)[RF], char* stage, const i
 // u[part][t][r].  grid (parts, rows or slots: the parts fastest, since blocks go round the eight dies and of a window's slots the first few alone have tiles)
 template <typename P, bool WHOLE, int RF, int TF, int KB, int AHEAD>
 __global__ __launch_bounds__(256) void adapter_down_kernel(float* __restrict__ u, const typename El<P>::type* __restrict__ x, const typename El<P>::type* __restrict__ a,
-                                                           const int* __restrict__ adapter, const int* __restrict__ rank, const int* __restrict__ plan, int slots,
+                                                           const int* __restrict__ adapter, const int* __restrict__ rank, int* __restrict__ plan, int slots,
                                                            int T, int K, int S, int R, int per) {
   __shared__ int rows[16 * TF], waves[5];
   __shared__ __attribute__((aligned(16))) char stage[Down<P, RF, TF, KB>::ROOM];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  __shared__ int own_plan[TF == 1 ? 1 : PLAN_INTS];
+  static_assert(TF == 1 || sizeof(PlanRoom) <= sizeof stage);
   const Place at = place_of<TF>();
   const int k0 = at.x * per, k1 = min(K, k0 + per);
-  each_tile<TF>(at.y, plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
+  if constexpr (TF > 1) {
+    plan_window(own_plan, *reinterpret_cast<PlanRoom*>(stage), at.y / slots, adapter, T, S);
+    __syncthreads();
+    if (at.x == 0 && at.y % slots == 0)
+      for (int i = threadIdx.x; i < PLAN_INTS; i += 256) plan[(long)(at.y / slots) * PLAN_INTS + i] = own_plan[i];
+  }
+  each_tile<TF>(at.y, own_plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
     if (tile.adapter < 0) return;
     const int ra = rank ? min(max(rank[tile.adapter], 0), R) : R;
     if (ra < 1) return;
@@ -271,7 +299,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float
   const int row = threadIdx.x / PER_ROW, quad = threadIdx.x % PER_ROW;
   const Place at = place_of<TF>();
   const int n0 = at.x * columns, n1 = min(N, n0 + columns);
-  each_tile<TF>(at.y, plan, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
+  each_tile<TF>(at.y, TF == 1 ? plan : plan + (long)(at.y / slots) * PLAN_INTS, slots, T, S, adapter, rows, waves, [&](const Tile tile) {
     const int ra = tile.adapter < 0 ? 0 : rank ? min(max(rank[tile.adapter], 0), R) : R;
     if (ra < 1 && out == base) return;
     f32x4 x[NB];
@@ -452,7 +480,8 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(float* out, const float
 // One token, bf16, 2048 x 2560, rank 8: 3.1 + 4.9 us by two launches, 6.8 by one; the whole call
 // 16.6 and 12.6.
 static bool adapter_fused(int T, int K, int R) { return T <= 64 && R <= 64 && (long)R * K <= 32768; }
-static int adapter_parts(int T, int K) { return std::max(1, std::min(T > 4096 ? 2 : T > 2048 ? 4 : 8, (K + 511) / 512)); }
+// pieces of K: more workgroups, and as many sums that the second product reads (1999 rows, 4096 x 4096, rank 32: 8 pieces 25.9 us, 4 24.9)
+static int adapter_parts(int T, int K) { return std::max(1, std::min(T > 4096 ? 2 : T > 1024 ? 4 : 8, (K + 511) / 512)); }
 static long plan_ints(int T) { return T > WINDOW ? (long)((T + WINDOW - 1) / WINDOW) * PLAN_INTS : 0; }
 
 extern "C" long umb_seq_adapters_floats(int T, int K, int R) {
@@ -469,11 +498,11 @@ static int adapters_launch(float* out, const float* base, const void* x, const v
   if (TF > 1) {
     plan = reinterpret_cast<int*>(u + (((long)parts * T * R + 3) & ~3L));
     const int windows = (T + WINDOW - 1) / WINDOW;
-    slots = T <= 2048 ? 32 : 8;
+    // A window of few adapters has some five tiles; of many one each and more.  Blocks without a tile cost the making of a plan, blocks of several take them in turn (us:
+    // 1000 rows of 8 adapters in any order 8 slots 20, 16 29; of 64 8 slots 77, 16 68, 32 61; 300 rows of 64 58, 33, 20; beyond 2048 rows all blocks are busy).
+    slots = T > 2048 || S <= 8 ? 8 : 32;
     blocks = windows * slots;
     tiles = (T + PLAN_TILE - 1) / PLAN_TILE;
-    hipLaunchKernelGGL(adapter_plan_kernel, dim3(windows), dim3(64), 0, st, plan, adapter, T, S);
-    UMB_LAUNCH_CHECK();
   }
   int columns = 256;
   while (columns < 1024 && (long)tiles * (N / (2 * columns)) >= 1024) columns *= 2;
