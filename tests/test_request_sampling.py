@@ -69,7 +69,8 @@ def test_every_setting(V, spread):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,V", [(1, 151936), (130, 5000), (300, 777), (2, 524288)])
+@pytest.mark.parametrize("rows,V", [(1, 151936), (130, 5000), (300, 777), (2, 524288), (9, 1024), (9, 1025), (9, 8192), (9, 8193), (9, 16384), (9, 16385), (66, 20001), (66, 32768),
+                                    (65, 32769)])
 def test_rows_and_vocabularies(rows, V):
     x = torch.randn(rows, V, generator=torch.Generator().manual_seed(rows)) * 3
     check(x, **draws(rows, 5))

@@ -7,7 +7,7 @@
 // Weights are 64-bit floats, summed as whole numbers: such sums are the same in any order, and a border between two tokens falls where a 64-bit sum of
 // any order puts it but for some 1e-12 of the mass.  (In 32 bits a flat row of 128256 values has thousands of borders that the sum's order moves.)
 //
-// Nothing is sorted but what stands next to a border.  Three launches:
+// Nothing is sorted but what stands next to a border.  Three launches (two for rows of one slice):
 //   slices   a row in slices, each read once into registers: its largest, and counts and masses of bins T / 32 wide, 1024 below the largest (what is
 //            further down weighs less than 2^-46 of the row).  Bins lie on one lattice, floor(32 x / T), and masses are relative to their bin's middle, so
 //            that slices' add up as whole numbers, count and mass in one 64-bit atomic
@@ -18,7 +18,7 @@
 // us (slices, collect, resolve): a row of 32000 3.8, 8, 9.9; 8 of 128256 5.2, 11.3, 10.2; 48 of 151936 12.2, 19.6, 16.6; 256 of 128256 37.4, 29.4, 14.
 // Bound by the logits where rows are many: the first launch reads them from memory, the second once more, from the cache behind it; by launches and barriers where
 // they are few.
-// Rows of up to SMALL_V values are taken whole by the last launch alone.  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
+// Rows of up to SMALL_V values are taken whole by the last launch alone (1000 values 15 - 17 us, 1500 20 against 16 - 18 by two).  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
 // the thousand), is searched eight bits of the key at a time, by one workgroup.
 #include "seq_common.h"
 #include <algorithm>
@@ -188,7 +188,7 @@ __device__ __attribute__((noinline)) void sample_slow(int r, int* __restrict__ t
 }
 
 // ------------------------------------------------------------------ bins
-constexpr int BINS = 1024, SMALL_V = 2048, CAP = 2048, K_COUNT = 1024, P_MAX = 64, FEW = 128;
+constexpr int BINS = 1024, SMALL_V = 1024, CAP = 2048, K_COUNT = 1024, P_MAX = 64, FEW = 128;
 constexpr double PER_T = 32.0, LATTICE = 1099511627776.0;         // bins a T; beyond 2^40 neighbouring floats are 2^16 bins apart and more
 constexpr double MAGIC = 4503599627370496.0;                     // 2^52: added to a number below 2^51, it leaves the nearest whole number in the low bits
 constexpr double BIN_ONE = 4294967296.0;                         // a bin's masses, in 2^-32 of its middle's weight: 48 bits for 2^15 of them, 16 above for their number
@@ -272,12 +272,13 @@ struct RowSums {
 static_assert(sizeof(RowSums) % 16 == 0 && sizeof(RowSaid) % 16 == 0);
 // How a row is cut: slices of `slice` values (P), which the first launch counts; chunks of `chunk` values, every Q-th of which the second launch's block q looks
 // through, with room for a quarter of them.  Few rows: as many workgroups as there are pieces of 8192; many: larger pieces, and as many workgroups as stay
-// resident, since each adds up its row's bins first.
+// resident, since each adds up its row's bins first.  Rows of one slice take the second launch alone, which makes their bins (us: 8192 values 19.5 -> 16, 256 rows
+// of 12000 32 -> 22; up to 32768 where the rows keep the chip busy: 32000 values 64 rows 27.6 either way, 256 rows 39 -> 29.5, one 20.4 -> 20.7).
 struct Cut { int slice, P, chunk, Q, cap; };
 static Cut cut_of(int rows, int V) {
   const bool few = (long)rows * ((V + 8191) / 8192) <= 512;
   Cut c;
-  c.slice = c.chunk = few ? 8192 : 16384;
+  c.slice = c.chunk = V <= 8192 ? 8192 : V <= 16384 ? 16384 : V <= 32768 && rows > 64 ? 32768 : few ? 8192 : 16384;
   c.P = (V + c.slice - 1) / c.slice;
   c.Q = few ? c.P : std::max(1, std::min(c.P, 512 / rows));
   c.cap = (c.P + c.Q - 1) / c.Q * (c.chunk / 4);
@@ -324,6 +325,32 @@ template <int NT, int NE, bool VEC> __device__ __forceinline__ void load_slice(f
   for (int e = 0; e < NE; ++e) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
 }
 
+// counts and masses of a slice's values, whose largest is `top`
+template <int NE> __device__ __forceinline__ void bin_slice(const float (&x)[NE], unsigned long long* bins, float top, double per, int k) {
+  const double first = floor(line_of(top, per));
+  if (top == INFINITY || !(fabs((double)top * per) < LATTICE)) {   // its equals alone count
+#pragma unroll
+    for (int e = 0; e < NE; ++e) if (x[e] == top) atomicAdd(bins, 1ull << 48);
+  } else if (k >= 1 && k <= K_COUNT) {
+    // (-inf, and what the lattice does not reach, are far below)
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const double j = first - floor((double)x[e] * per);
+      const int at = (int)j;
+      if (j < BINS) atomicAdd(reinterpret_cast<unsigned*>(bins + at) + 1, 1u << 16);
+    }
+  } else {
+    const BinExp weight;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {           // (worked out for all, so that elements run side by side)
+      const double l = (double)x[e] * per, f = floor(l), j = first - f;
+      const int at = (int)j;
+      const unsigned long long v = (1ull << 48) + weight(l - f);
+      if (j < BINS) atomicAdd(bins + at, v);
+    }
+  }
+}
+
 // grid (slices, rows)
 template <int NT, int NE, bool VEC>
 __global__ __launch_bounds__(NT) void sample_slices_kernel(char* __restrict__ scratch, Cut cut, const float* __restrict__ logits, long ld, int V,
@@ -353,29 +380,7 @@ __global__ __launch_bounds__(NT) void sample_slices_kernel(char* __restrict__ sc
   }
   if (threadIdx.x == 0) s.heads[p] = SliceHead{top, at, {0, 0}};
   if (!(top > -INFINITY) || !(t > 0.f)) return;
-  const double per = PER_T / (double)t, first = floor(line_of(top, per));
-  const int k = top_k ? top_k[r] : 0;
-  if (top == INFINITY || !(fabs((double)top * per) < LATTICE)) {   // its equals alone count
-#pragma unroll
-    for (int e = 0; e < NE; ++e) if (x[e] == top) atomicAdd(bins, 1ull << 48);
-  } else if (k >= 1 && k <= K_COUNT) {
-    // (-inf, and what the lattice does not reach, are far below)
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      const double j = first - floor((double)x[e] * per);
-      const int at = (int)j;
-      if (j < BINS) atomicAdd(reinterpret_cast<unsigned*>(bins + at) + 1, 1u << 16);
-    }
-  } else {
-    const BinExp weight;
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {           // (worked out for all, so that elements run side by side)
-      const double l = (double)x[e] * per, f = floor(l), j = first - f;
-      const int at = (int)j;
-      const unsigned long long v = (1ull << 48) + weight(l - f);
-      if (j < BINS) atomicAdd(bins + at, v);
-    }
-  }
+  bin_slice<NE>(x, bins, top, PER_T / (double)t, top_k ? top_k[r] : 0);
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += NT) s.bins[p * BINS + i] = bins[i];
 }
@@ -447,48 +452,75 @@ __device__ __forceinline__ Two how_many(bool a, bool b, int* cell, bool also_a =
   return Two{w & 0xffff, w >> 16};
 }
 
-// grid (Q, rows); a thread a bin
-template <int NE, bool VEC>
-__global__ __launch_bounds__(BINS, 8) void sample_collect_kernel(char* __restrict__ scratch, Cut cut, const float* __restrict__ logits, long ld, int V,
+// grid (Q, rows); a thread a bin.  ONE: rows of one slice, whose bins are made here too
+template <int NE, bool VEC, bool ONE>
+__global__ __launch_bounds__(BINS, NE > 16 ? 4 : 8) void sample_collect_kernel(char* __restrict__ scratch, Cut cut, const float* __restrict__ logits, long ld, int V,
                                                               const float* __restrict__ uniforms, const float* __restrict__ temperature, const int* __restrict__ top_k,
                                                               const float* __restrict__ top_p, const float* __restrict__ min_p) {
   constexpr int NT = BINS;
   __shared__ double m_in[BINS], wave_m[NT / 64];
   __shared__ int shift[P_MAX], c_in[BINS], wave_c[NT / 64], cells[3], found;
-  __shared__ float bounds[4][2];
+  __shared__ float bounds[4][2], tops[NT / 64];
+  __shared__ unsigned long long bins[ONE ? BINS : 1];
+  __shared__ int at_top;
   const int r = blockIdx.y, P = cut.P, b = threadIdx.x, lane = b & 63;
   int p = blockIdx.x;                        // chunk
   const RowSettings set = row_settings(r, V, temperature, top_k, top_p, min_p, uniforms);
-  if (set.greedy) return;
+  if (!ONE && set.greedy) return;
   const Scratch s = scratch_of(scratch, r, cut);
   float x[NE];                               // (asked for early: what comes in between is latency)
   load_slice<NT, NE, VEC>(x, logits + (long)r * ld, p * NT * NE, V);
-  const float head = lane < P ? s.heads[lane].top : -INFINITY, top = wave_max(head);
+  float head = -INFINITY, top;
+  if constexpr (ONE) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) head = fmaxf(head, x[e]);
+    head = wave_max(head);
+    if (lane == 0) tops[b >> 6] = head;
+    bins[b] = 0ull;
+    if (b == 0) at_top = 0x7fffffff;
+    __syncthreads();
+    top = wave_max(tops[lane & (NT / 64 - 1)]);
+    if (set.greedy) {                        // the first of the largest
+#pragma unroll
+      for (int e = 0; e < NE; ++e) if (x[e] == top) atomicMin(&at_top, index_of<NT, NE, VEC>(0, e));
+      __syncthreads();
+    }
+    if (b == 0) s.heads[0] = SliceHead{top, at_top, {0, 0}};
+    if (set.greedy) return;
+  } else {
+    head = lane < P ? s.heads[lane].top : -INFINITY;
+    top = wave_max(head);
+  }
   if (!(top > -INFINITY)) return;
   const double per = PER_T / set.t, line = line_of(top, per), first = floor(line);
-  if (b < P) {
+  if (!ONE && b < P) {
     const double d = first - floor(line_of(head, per));
     shift[b] = d < BINS && counts(head, top, per) ? (int)d : BINS;
   }
   if (b == 0) found = 0;
   if (b < 3) cells[b] = 0;
+  if constexpr (ONE) bin_slice<NE>(x, bins, top, per, top_k ? top_k[r] : 0);
   __syncthreads();
   unsigned long long q = 0ull;
   int c = 0;
   constexpr int BATCH = NE <= 8 ? 16 : 8;    // slices asked for together
-  for (int i0 = 0; i0 < P; i0 += BATCH) {
-    unsigned long long v[BATCH];
+  if constexpr (ONE) {
+    c = (int)(bins[b] >> 48);
+    q = bins[b] & 0xffffffffffffull;
+  } else
+    for (int i0 = 0; i0 < P; i0 += BATCH) {
+      unsigned long long v[BATCH];
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int k = i0 + i < P ? b - shift[i0 + i] : -1;
-      v[i] = k >= 0 ? s.bins[(i0 + i) * BINS + k] : 0ull;
-    }
+      for (int i = 0; i < BATCH; ++i) {
+        const int k = i0 + i < P ? b - shift[i0 + i] : -1;
+        v[i] = k >= 0 ? s.bins[(i0 + i) * BINS + k] : 0ull;
+      }
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      c += (int)(v[i] >> 48);
-      q += v[i] & 0xffffffffffffull;
+      for (int i = 0; i < BATCH; ++i) {
+        c += (int)(v[i] >> 48);
+        q += v[i] & 0xffffffffffffull;
+      }
     }
-  }
   // a bin's middle beside the largest; beside an infinite one, or one beyond the lattice, only its equals count
   const bool flat = top == INFINITY || !(fabs((double)top * per) < LATTICE);
   double m = flat ? (b == 0 ? (double)c : 0.0) : (double)q * (1.0 / BIN_ONE) * exp_down((first - b + 0.5 - line) * (1.0 / PER_T));
@@ -1047,14 +1079,23 @@ extern "C" int umb_sample_requests(int* tokens, float* probs, const float* logit
     char* const sc = static_cast<char*>(scratch) + r0 * row_bytes(cut);
     const float* const x = logits + r0 * ld;
     auto at = [&](auto* p) { return p ? p + r0 : p; };
+#define ONE_SLICE(NE, VEC)                                                                                                                       \
+  hipLaunchKernelGGL((sample_collect_kernel<NE, VEC, true>), dim3(1, n), dim3(BINS), 0, st, sc, cut, x, ld, V, at(uniforms), at(temperature), at(top_k), \
+                     at(top_p), at(min_p))
 #define SLICES(NT, NE, VEC)                                                                                                                         \
   hipLaunchKernelGGL((sample_slices_kernel<NT, NE, VEC>), dim3(cut.P, n), dim3(NT), 0, st, sc, cut, x, ld, V, at(temperature), at(top_k));           \
-  hipLaunchKernelGGL((sample_collect_kernel<NT * NE / BINS, VEC>), dim3(cut.Q, n), dim3(BINS), 0, st, sc, cut, x, ld, V, at(uniforms), at(temperature), \
-                     at(top_k), at(top_p), at(min_p))
-    if (cut.slice == 8192 && vec) { SLICES(512, 16, true); }
+  hipLaunchKernelGGL((sample_collect_kernel<NT * NE / BINS, VEC, false>), dim3(cut.Q, n), dim3(BINS), 0, st, sc, cut, x, ld, V, at(uniforms),        \
+                     at(temperature), at(top_k), at(top_p), at(min_p))
+    if (cut.P == 1) {
+      if (cut.slice == 8192) { if (vec) ONE_SLICE(8, true); else ONE_SLICE(8, false); }
+      else if (cut.slice == 16384) { if (vec) ONE_SLICE(16, true); else ONE_SLICE(16, false); }
+      else { if (vec) ONE_SLICE(32, true); else ONE_SLICE(32, false); }
+    }
+    else if (cut.slice == 8192 && vec) { SLICES(512, 16, true); }
     else if (cut.slice == 8192) { SLICES(512, 16, false); }
     else if (vec) { SLICES(512, 32, true); }
     else { SLICES(512, 32, false); }
+#undef ONE_SLICE
 #undef SLICES
     hipLaunchKernelGGL((sample_resolve_kernel<false>), dim3(n), dim3(ST), 0, st, at(tokens), at(probs), sc, cut, x, ld, V, at(uniforms), at(temperature), at(top_k),
                        at(top_p), at(min_p));
