@@ -204,3 +204,36 @@ def test_refusals_of_the_entry_point(kw):
     n = lib.umb_sample_requests_bytes(3, 64) if a["scratch_bytes"] is None else a["scratch_bytes"]
     assert lib.umb_sample_requests_bytes(0, 64) == 0 and lib.umb_sample_requests_bytes(3, 0) == 0 and lib.umb_sample_requests_bytes(1, MAX_VOCAB + 1) == 0
     assert lib.umb_sample_requests(a["tokens"], None, a["logits"], a["ld"], a["rows"], a["V"], a["uniforms"], None, None, None, None, a["scratch"], n, None) == EINVAL
+
+
+def check_finely(x, u, t, k, p, m):
+    """check, with sums in 80 bits: in 64, half a million additions of 1e-11 to 1 are off by whole tokens themselves (2^-53 each, 524288 of them 6e-11: four tokens)"""
+    got = sample_rows(x.cuda(), *(torch.tensor(v, dtype=torch.float32).cuda() for v in (u, t)), top_k=torch.tensor(k, dtype=torch.int32).cuda(),
+                      top_p=torch.tensor(p, dtype=torch.float32).cuda(), min_p=torch.tensor(m, dtype=torch.float32).cuda())
+    want, shares = [], []
+    for r in range(x.shape[0]):
+        v = x[r].numpy().astype(np.longdouble)
+        order = np.lexsort((np.arange(v.size), -v))
+        order = order[v[order] > -INF]
+        w = np.exp((v[order] - v[order[0]]) / np.longdouble(np.float32(t[r])))
+        w = w[:k[r]] if k[r] > 0 else w
+        upto = np.cumsum(w)
+        n = min(int((np.concatenate([[0.0], upto[:-1]]) < np.longdouble(np.float32(p[r])) * upto[-1]).sum()) if p[r] < 1 else w.size, int((w >= np.float32(m[r])).sum()))
+        at = min(int((upto[:n] <= np.longdouble(np.float32(u[r])) * upto[n - 1]).sum()), n - 1)
+        want.append(int(order[at])), shares.append(float(w[at] / upto[n - 1]))
+    assert got[0].tolist() == want
+    shares = torch.tensor(shares, dtype=torch.float64)
+    assert bool(((got[1].cpu().double() - shares).abs() <= shares * (2.0 ** -24 + 1e-10)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,down", [(128256, 20.0), (262144, 18.0), (30000, 15.0), (524288, 25.0)])
+def test_draws_from_equal_logits_far_below_one(V, down):
+    """a share of 1e-4 and less in tokens of 1e-9 each: u counts them off"""
+    x = torch.full((1, V), 3.0 - down)
+    x[0, V // 3] = 3.0
+    share = (V - 1) * np.exp(-down) / (1 + (V - 1) * np.exp(-down))
+    u = [0.99975723] if V == 128256 else []
+    u += [1.0 - share * f for f in np.linspace(0.01, 0.99, 40)]
+    r = len(u)
+    check_finely(x.expand(r, V).contiguous(), u, [1.0] * r, [0] * r, [1.0] * r, [0.0] * r)

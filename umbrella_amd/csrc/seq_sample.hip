@@ -19,12 +19,13 @@
 // Bound by the logits where rows are many: the first launch reads them from memory, the second once more, from the cache behind it; by launches and barriers where
 // they are few.
 // Rows of up to SMALL_V values are taken whole by the last launch alone (1000 values 15 - 17 us, 1500 20 against 16 - 18 by two).  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
-// the thousand), is searched eight bits of the key at a time, by one workgroup.
+// the thousand), is searched eight bits of the key at a time, by one workgroup, four passes a border (ms: 128256 equal values 1.1, 2.0 with a p, 2.9 with a k too; 48 rows
+// of as many rounded to whole numbers, with a p, 1.25).
 #include "seq_common.h"
 #include <algorithm>
 
-constexpr int SAMPLE_VMAX = 1 << 19;         // 2^19 weights of at most 2^44 are a number of 63 bits
-constexpr double MASS_ONE = 17592186044416.0;
+constexpr int SAMPLE_VMAX = 1 << 19;         // a Mass holds so many
+constexpr double MAGIC = 4503599627370496.0; // 2^52: added to a number below 2^51, it leaves the nearest whole number in the low bits
 
 // NaN counts as -inf; larger values have larger keys
 __device__ __forceinline__ unsigned key_of(float x) {
@@ -40,7 +41,21 @@ __device__ __forceinline__ double weight_of(unsigned key, float top, double t) {
   const float x = of_key(key);
   return key <= KEY_NONE ? 0.0 : x == top ? 1.0 : top < INFINITY ? exp(((double)x - (double)top) / t) : 0.0;
 }
-__device__ __forceinline__ unsigned long long mass_of(double w) { return (unsigned long long)(w * MASS_ONE + 0.5); }
+// A sum of weights of at most 1 in whole numbers, the same in any order: of 2^-40, and of what each weight's rounding to those leaves, of 2^-84.  2^19 of them
+// are good to 2^-66.  (In 2^-44 alone, 128255 tokens of 2e-9 beside one of 1 were 1e-9 off together, and every third draw among them the token beside the right one.)
+struct Mass {
+  unsigned long long hi;
+  long long lo;
+  __device__ __forceinline__ double value() const { return (double)hi * (1.0 / 1099511627776.0) + (double)lo * (1.0 / 19342813113834066795298816.0); }
+  __device__ __forceinline__ Mass operator+(const Mass& o) const { return Mass{hi + o.hi, lo + o.lo}; }
+  __device__ __forceinline__ Mass operator-(const Mass& o) const { return Mass{hi - o.hi, lo - o.lo}; }
+  __device__ __forceinline__ Mass operator*(int n) const { return Mass{hi * (unsigned long long)n, lo * n}; }
+};
+__device__ __forceinline__ Mass mass_of(double w) {
+  const double ONE = 1099511627776.0, REST = 17592186044416.0, HALF = 1.5 * MAGIC;
+  const double h = fma(w, ONE, MAGIC), l = fma(fma(w, ONE, MAGIC - h), REST, HALF);            // (both differences are exact)
+  return Mass{(unsigned long long)__double_as_longlong(h) & 0xfffffffffffffull, __double_as_longlong(l) - __double_as_longlong(HALF)};
+}
 
 struct RowSettings { double t, p, m, u; int k; bool greedy; };
 __device__ __forceinline__ RowSettings row_settings(int row, int V, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
@@ -61,7 +76,14 @@ constexpr int ST = 1024;
 struct Pick {                                // the element that a search ended at: its key, its place among its equals, what stands in front of those
   unsigned key;
   int tie, count;
-  unsigned long long mass;
+  Mass mass;
+};
+// LDS of the searches; sums of a digit's masses, and of everything (0) and of what min-p keeps (1)
+struct SlowRoom {
+  unsigned cnt[256];
+  unsigned long long hi[256], lo[256], wide[6];
+  Mass front;
+  int digit, count, tie;
 };
 
 // The first element, in order, at which what has come up to and with it reaches a goal: BY_COUNT the goal-th element; otherwise the first whose
@@ -69,58 +91,60 @@ struct Pick {                                // the element that a search ended 
 // Four passes over the row, eight bits of the key each.
 enum { BY_COUNT, AT_LEAST, OVER };
 template <int HOW>
-__device__ Pick find_in_row(const float* __restrict__ row, int V, float top, double t, double goal, unsigned* cnt, unsigned long long* sum, int* shared) {
-  Pick got{0u, 0, 0, 0ull};
+__device__ Pick find_in_row(const float* __restrict__ row, int V, float top, double t, double goal, SlowRoom& room) {
+  Pick got{0u, 0, 0, Mass{0ull, 0ll}};
   unsigned mask = 0u;
   auto reached = [&](double n, double q) { return HOW == BY_COUNT ? n >= goal : HOW == AT_LEAST ? q >= goal : q > goal; };
   for (int shift = 24; shift >= 0; shift -= 8) {
     __syncthreads();
-    if (threadIdx.x < 256) { cnt[threadIdx.x] = 0u; sum[threadIdx.x] = 0ull; }
+    if (threadIdx.x < 256) { room.cnt[threadIdx.x] = 0u; room.hi[threadIdx.x] = room.lo[threadIdx.x] = 0ull; }
     __syncthreads();
     for (int i = threadIdx.x; i < V; i += ST) {
       const unsigned k = key_of(row[i]);
       if ((k & mask) == got.key && k > KEY_NONE) {
         const int d = (k >> shift) & 255;
-        atomicAdd(&cnt[d], 1u);
-        const unsigned long long q = mass_of(weight_of(k, top, t));
-        if (q) atomicAdd(&sum[d], q);
+        atomicAdd(&room.cnt[d], 1u);
+        const Mass q = mass_of(weight_of(k, top, t));
+        if (q.hi) atomicAdd(&room.hi[d], q.hi);
+        if (q.lo) atomicAdd(&room.lo[d], (unsigned long long)q.lo);
       }
     }
     __syncthreads();
     if (threadIdx.x == 0) {
       int n = got.count, d = 255, last = -1;
-      unsigned long long q = got.mass;
+      Mass q = got.mass;
+      auto of = [&](int i) { return Mass{room.hi[i], (long long)room.lo[i]}; };
       for (; d >= 0; --d) {
-        if (!cnt[d]) continue;
-        if (reached((double)(n + cnt[d]), (double)(q + sum[d]))) break;
+        if (!room.cnt[d]) continue;
+        if (reached((double)(n + room.cnt[d]), (q + of(d)).value())) break;
         last = d;
-        n += cnt[d];
-        q += sum[d];
+        n += room.cnt[d];
+        q = q + of(d);
       }
-      if (d < 0) { d = last < 0 ? 0 : last; n -= cnt[d]; q -= sum[d]; }
-      shared[0] = d;
-      shared[1] = n;
-      reinterpret_cast<unsigned long long*>(shared)[1] = q;
+      if (d < 0) { d = last < 0 ? 0 : last; n -= room.cnt[d]; q = q - of(d); }
+      room.digit = d;
+      room.count = n;
+      room.front = q;
     }
     __syncthreads();
-    got.key |= (unsigned)shared[0] << shift;
-    got.count = shared[1];
-    got.mass = reinterpret_cast<unsigned long long*>(shared)[1];
+    got.key |= (unsigned)room.digit << shift;
+    got.count = room.count;
+    got.mass = room.front;
     mask |= 255u << shift;
     if (shift == 0) {                        // equals, in the order of their indices
-      const int n = cnt[shared[0]];
-      const unsigned long long q = mass_of(weight_of(got.key, top, t));
+      const int n = room.cnt[room.digit];
+      const Mass q = mass_of(weight_of(got.key, top, t));
       if (threadIdx.x == 0) {
         int lo = 0, hi = n - 1;
         while (lo < hi) {
           const int mid = (lo + hi) >> 1;
-          if (reached((double)(got.count + mid + 1), (double)(got.mass + q * (mid + 1)))) hi = mid;
+          if (reached((double)(got.count + mid + 1), (got.mass + q * (mid + 1)).value())) hi = mid;
           else lo = mid + 1;
         }
-        shared[4] = lo;
+        room.tie = lo;
       }
       __syncthreads();
-      got.tie = shared[4];
+      got.tie = room.tie;
     }
   }
   __syncthreads();
@@ -128,45 +152,46 @@ __device__ Pick find_in_row(const float* __restrict__ row, int V, float top, dou
 }
 
 // the whole of a row by one workgroup, some eleven passes over it
-struct SlowRoom { unsigned cnt[256]; unsigned long long sum[256]; unsigned long long wide[16]; int shared[8]; };
 __device__ __attribute__((noinline)) void sample_slow(int r, int* __restrict__ tokens, float* __restrict__ probs, const float* __restrict__ row, int V, RowSettings s,
                                                       float top, SlowRoom& room) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  unsigned* cnt = room.cnt;
-  unsigned long long *sum = room.sum, *wide = room.wide;
-  int* shared = room.shared;
+  unsigned long long* wide = room.wide;
   // everything's and min-p's counts and masses
   __syncthreads();
-  if (tid < 4) wide[tid] = 0ull;
+  if (tid < 6) wide[tid] = 0ull;
   __syncthreads();
-  unsigned long long n_all = 0, q_all = 0, n_min = 0, q_min = 0;
+  unsigned long long n_all = 0, n_min = 0;
+  Mass q_all{0ull, 0ll}, q_min{0ull, 0ll};
   for (int i = tid; i < V; i += ST) {
     const unsigned k = key_of(row[i]);
     const double w = weight_of(k, top, s.t);
-    const unsigned long long q = mass_of(w);
-    if (k > KEY_NONE) { ++n_all; q_all += q; if (w >= s.m) { ++n_min; q_min += q; } }
+    const Mass q = mass_of(w);
+    if (k > KEY_NONE) { ++n_all; q_all = q_all + q; if (w >= s.m) { ++n_min; q_min = q_min + q; } }
   }
   atomicAdd(&wide[0], n_all);
-  atomicAdd(&wide[1], q_all);
-  atomicAdd(&wide[2], n_min);
-  atomicAdd(&wide[3], q_min);
+  atomicAdd(&wide[1], q_all.hi);
+  atomicAdd(&wide[2], (unsigned long long)q_all.lo);
+  atomicAdd(&wide[3], n_min);
+  atomicAdd(&wide[4], q_min.hi);
+  atomicAdd(&wide[5], (unsigned long long)q_min.lo);
   __syncthreads();
   n_all = wide[0];
-  q_all = wide[1];
-  long n = (long)wide[2];
-  unsigned long long q = wide[3];
+  q_all = Mass{wide[1], (long long)wide[2]};
+  long n = (long)wide[3];
+  Mass q{wide[4], (long long)wide[5]};
   if (n < 1) { n = 1; q = mass_of(1.0); }
-  unsigned long long q_k = q_all;
+  Mass q_k = q_all;
   if ((unsigned long long)s.k < n_all) {
-    const Pick e = find_in_row<BY_COUNT>(row, V, top, s.t, (double)s.k, cnt, sum, shared);
+    const Pick e = find_in_row<BY_COUNT>(row, V, top, s.t, (double)s.k, room);
     q_k = e.mass + mass_of(weight_of(e.key, top, s.t)) * (e.tie + 1);
     if (s.k < n) { n = s.k; q = q_k; }
   }
   if (s.p < 1.0) {
-    const Pick e = find_in_row<AT_LEAST>(row, V, top, s.t, fmax(s.p, 0.0) * (double)q_k, cnt, sum, shared);
+    const Pick e = find_in_row<AT_LEAST>(row, V, top, s.t, fmax(s.p, 0.0) * q_k.value(), room);
     if (e.count + e.tie + 1 < n) { n = e.count + e.tie + 1; q = e.mass + mass_of(weight_of(e.key, top, s.t)) * (e.tie + 1); }
   }
-  const Pick e = find_in_row<OVER>(row, V, top, s.t, s.u * (double)q, cnt, sum, shared);
+  const double mass = q.value();
+  const Pick e = find_in_row<OVER>(row, V, top, s.t, s.u * mass, room);
   // the tie-th of the values equal to e's, by index
   int seen = 0;
   for (int i0 = 0; i0 < V; i0 += ST) {
@@ -174,13 +199,13 @@ __device__ __attribute__((noinline)) void sample_slow(int r, int* __restrict__ t
     const bool is = i < V && key_of(row[i]) == e.key;
     const unsigned long long bal = __ballot(is);
     __syncthreads();
-    if (lane == 0) cnt[wave] = __popcll(bal);
+    if (lane == 0) room.cnt[wave] = __popcll(bal);
     __syncthreads();
     int before = seen, all = seen;
-    for (int w = 0; w < ST / 64; ++w) { if (w < wave) before += cnt[w]; all += cnt[w]; }
+    for (int w = 0; w < ST / 64; ++w) { if (w < wave) before += room.cnt[w]; all += room.cnt[w]; }
     if (is && before + __popcll(bal & ((1ull << lane) - 1ull)) == e.tie) {
       tokens[r] = i;
-      if (probs) probs[r] = (float)(weight_of(e.key, top, s.t) * MASS_ONE / (double)q);
+      if (probs) probs[r] = (float)(weight_of(e.key, top, s.t) / mass);
     }
     seen = all;
     if (seen > e.tie) break;
@@ -190,7 +215,6 @@ __device__ __attribute__((noinline)) void sample_slow(int r, int* __restrict__ t
 // ------------------------------------------------------------------ bins
 constexpr int BINS = 1024, SMALL_V = 1024, CAP = 2048, K_COUNT = 1024, P_MAX = 64, FEW = 128;
 constexpr double PER_T = 32.0, LATTICE = 1099511627776.0;         // bins a T; beyond 2^40 neighbouring floats are 2^16 bins apart and more
-constexpr double MAGIC = 4503599627370496.0;                     // 2^52: added to a number below 2^51, it leaves the nearest whole number in the low bits
 constexpr double BIN_ONE = 4294967296.0;                         // a bin's masses, in 2^-32 of its middle's weight: 48 bits for 2^15 of them, 16 above for their number
 constexpr double FINE_ONE = 70368744177664.0;                    // 2^46, of the row's largest weight
 
