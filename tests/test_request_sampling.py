@@ -237,3 +237,22 @@ def test_draws_from_equal_logits_far_below_one(V, down):
     u += [1.0 - share * f for f in np.linspace(0.01, 0.99, 40)]
     r = len(u)
     check_finely(x.expand(r, V).contiguous(), u, [1.0] * r, [0] * r, [1.0] * r, [0.0] * r)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,n,settings", [(1000, 999, ((0, 0.0), (1000, 0.0), (0, 1e-12))), (40000, 900, ((901, 0.0), (901, 1e-12)))])
+def test_draws_from_few_logits_far_below_one(V, n, settings):
+    """the same among tokens that are all put in order, at every u that is in the tail"""
+    x, u = [], []
+    for i in range(0, 300, 1 if V < 2000 else 4):
+        down = float(np.float32(21 + 0.01 * i))
+        share = n * np.exp(-down) / (1 + n * np.exp(-down))
+        row = torch.full((V,), -INF)
+        row[V // 2 - n // 2:V // 2 - n // 2 + n + 1] = -down
+        row[V // 2] = 0.0
+        for k in range(1, 13):
+            if k * 2.0 ** -24 < share:
+                x.append(row), u.append(1.0 - k * 2.0 ** -24)
+    x, r = torch.stack(x), len(u)
+    for k, m in settings:
+        check_finely(x, u, [1.0] * r, [k] * r, [1.0] * r, [m] * r)

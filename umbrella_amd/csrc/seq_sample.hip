@@ -216,7 +216,10 @@ __device__ __attribute__((noinline)) void sample_slow(int r, int* __restrict__ t
 constexpr int BINS = 1024, SMALL_V = 1024, CAP = 2048, K_COUNT = 1024, P_MAX = 64, FEW = 128;
 constexpr double PER_T = 32.0, LATTICE = 1099511627776.0;         // bins a T; beyond 2^40 neighbouring floats are 2^16 bins apart and more
 constexpr double BIN_ONE = 4294967296.0;                         // a bin's masses, in 2^-32 of its middle's weight: 48 bits for 2^15 of them, 16 above for their number
-constexpr double FINE_ONE = 70368744177664.0;                    // 2^46, of the row's largest weight
+// resolve's bins: in 2^-46 of a power of two that a bin's weights reach to half of at least, so that 2^17 of them are good to 2^-46 of what they weigh, however far down
+constexpr int FINE_BITS = 46;
+__device__ __forceinline__ int fine_shift(int bin) { return (max(bin - 1, 0) * 47273) >> 20; }            // log2 of e^((bin - 1) / 32), rounded down
+__device__ __forceinline__ double power_of_two(int e) { return __longlong_as_double((long long)(1023 + e) << 52); }
 
 // e^((f - 1/2) / 32) of 0 <= f < 1 in whole numbers of 1 / BIN_ONE: the polynomial of degree 4 that meets it in the five Chebyshev points, good to 5e-13 of it,
 // rounded by the addition of 2^52.  The coefficients are held in registers: as literals each costs two moves an element.
@@ -260,8 +263,8 @@ __device__ __forceinline__ double exp_down(double d) {
 __device__ __forceinline__ double weight_at(float x, float top, double inv_t) {
   return x == top ? 1.0 : top < INFINITY ? exp_down(((double)x - (double)top) * inv_t) : 0.0;
 }
-__device__ __forceinline__ unsigned long long fine_of(double w) {
-  return (unsigned long long)__double_as_longlong(fma(w, FINE_ONE, MAGIC)) & 0xfffffffffffffull;
+__device__ __forceinline__ unsigned long long fine_of(double w, int shift) {
+  return (unsigned long long)__double_as_longlong(fma(w, power_of_two(FINE_BITS + shift), MAGIC)) & 0xfffffffffffffull;
 }
 // whether a value weighs anything beside `top`, as far as infinities and the lattice's end tell
 __device__ __forceinline__ bool counts(float x, float top, double per) {
@@ -724,16 +727,17 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
                                                             const float* __restrict__ temperature, const int* __restrict__ top_k, const float* __restrict__ top_p,
                                                             const float* __restrict__ min_p) {
   typedef unsigned long long u64;
-  __shared__ __attribute__((aligned(16))) u64 v[CAP], raw[CAP];    // tokens; whole masses up to and with each
+  __shared__ __attribute__((aligned(16))) u64 v[CAP], raw[CAP];    // tokens; whole masses of bins, then masses (as 64-bit floats) in front of each bin, up to and with each token
   __shared__ double front_m[CAP];                                  // mass and count in front of each bin
   __shared__ int front_c[CAP], start[CAP];                         // where a bin's tokens start in v
   __shared__ u64 wide[ST / 64];
+  __shared__ double wide_m[ST / 64];
   __shared__ int narrow[ST / 64], cells[3];
   __shared__ short slot[BINS];
   __shared__ unsigned char want[CAP];
   __shared__ SlowRoom room;
   __shared__ int from[P_MAX + 1], got[4], ranks, taken, sum_c;
-  __shared__ u64 sum_m;
+  __shared__ Mass sum_m;
   __shared__ double masses;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* row = logits + (long)r * ld;
@@ -787,9 +791,12 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   bool whole = true, p_binds = set.p < 1.0, m_binds = set.m > 0.0 && set.m <= 1.0;
   const int k = set.m > 1.0 ? 1 : set.k;
   int m0 = 0, m1 = BINS - 1, found = 0;
-  static_assert(CAP * 8 >= BINS * 12 && BINS == ST);
+  static_assert(CAP * 8 >= BINS * 14 && BINS == ST);
+  auto mass_at = [&](int i) { return __longlong_as_double((long long)raw[i]); };
+  auto leave = [&](int i, double m) { raw[i] = (u64)__double_as_longlong(m); };
   double* const slot_m = reinterpret_cast<double*>(v);               // mass and count in front of each collected bin, while v holds no tokens
   int* const slot_c = reinterpret_cast<int*>(v + BINS);
+  short* const slot_bin = reinterpret_cast<short*>(slot_c + BINS);
   if constexpr (!SMALL) {
     if (__ballot(had > row_cut.cap)) {
       sample_slow(r, tokens, probs, row, V, set, top, room);
@@ -815,6 +822,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     if (found > FEW && bin_slot >= 0) {
       slot_m[bin_slot] = bin_m;
       slot_c[bin_slot] = bin_c;
+      slot_bin[bin_slot] = (short)tid;
     }
   }
   // (putting in order takes 13 us for 1024 tokens and more, 6 for 300, 1.6 for 64 and fewer; the bins and looking again 5, and a dozen tokens are left)
@@ -822,10 +830,11 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   // bins of the collected tokens: all in one (front of it nothing); those of collect; or `cut` in each of those
   int cut = 1;
   if (many) while (2 * cut * slots <= CAP && cut < 256) cut *= 2;
-  auto place = [&](u64 t) -> int {
+  auto place = [&](u64 t, int* shift = nullptr) -> int {
     if (SMALL || (whole && !many)) return 0;
     const double l = floor(line_of(value(t), per) * cut), c = floor(l * (1.0 / cut));
     const int j = max(0, min(BINS - 1, (int)(first - c)));
+    if (shift) *shift = fine_shift(j);
     return many ? max(0, (int)slot[j]) * cut + (cut - 1 - (int)(l - c * cut)) : j;
   };
   // f of each collected token, slice behind slice in memory; four loads of a thread in flight
@@ -847,12 +856,12 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   };
   if (tid < 4) got[tid] = CAP;
   if (tid < 3) cells[tid] = 0;
-  if (tid == 0) { taken = 0; sum_c = 0; sum_m = 0ull; }
+  if (tid == 0) { taken = 0; sum_c = 0; sum_m = Mass{0ull, 0ll}; }
   if (many) for (int i = tid; i < CAP; i += ST) { raw[i] = 0ull; start[i] = 0; }
   __syncthreads();
   // min-p's end: as many as weigh enough
   int count_m = 0;
-  u64 mass_m = 0ull;
+  Mass mass_m{0ull, 0ll};
   auto enough = [&](u64 t, double w) {
     if (!m_binds || !(w >= set.m) || (unsigned)(t >> 32) <= KEY_NONE) return;
     if (!SMALL && !whole) {
@@ -860,14 +869,15 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       if (j < m0 || j > m1) return;
     }
     ++count_m;
-    mass_m += fine_of(w);
+    mass_m = mass_m + mass_of(w);
   };
   if (many)
     each([&](int, u64 t) {
       const double w = token_weight(t);
       enough(t, w);
-      const int b = place(t);
-      atomicAdd(&raw[b], fine_of(w));
+      int shift;
+      const int b = place(t, &shift);
+      atomicAdd(&raw[b], fine_of(w, shift));
       atomicAdd(&start[b], 1);
     });
   else {
@@ -881,12 +891,15 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   if (m_binds) {
     if (__ballot(count_m > 0)) {
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) { mass_m += __shfl_xor(mass_m, o, 64); count_m += __shfl_xor(count_m, o, 64); }
-      if (lane == 0) { atomicAdd(&sum_m, mass_m); atomicAdd(&sum_c, count_m); }
+      for (int o = 32; o > 0; o >>= 1) {
+        mass_m = mass_m + Mass{__shfl_xor(mass_m.hi, o, 64), __shfl_xor(mass_m.lo, o, 64)};
+        count_m += __shfl_xor(count_m, o, 64);
+      }
+      if (lane == 0) { atomicAdd(&sum_m.hi, mass_m.hi); atomicAdd(reinterpret_cast<u64*>(&sum_m.lo), (u64)mass_m.lo); atomicAdd(&sum_c, count_m); }
     }
     __syncthreads();
     count_m = sum_c;
-    end_m = (double)sum_m * (1.0 / FINE_ONE);
+    end_m = sum_m.value();
     if (!SMALL && !whole) { count_m += s.sums->count[m0]; end_m += s.sums->mass[m0]; }
   }
   __syncthreads();
@@ -902,19 +915,20 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   if (many) {
     // each bin's sums, from those in front of it; then which bins the ends may lie in, as collect does
     const int b0 = 2 * tid;
-    const u64 q0 = raw[b0], q1 = raw[b0 + 1];
+    const int used = slots * cut;
+    auto mass_of_bin = [&](int b) { return b < used ? (double)raw[b] * power_of_two(-FINE_BITS - fine_shift(slot_bin[b / cut])) : 0.0; };
+    const double q0 = mass_of_bin(b0), q1 = mass_of_bin(b0 + 1);
     const int c0 = start[b0], c1 = start[b0 + 1];
-    u64 qs = q0 + q1;
+    double qs = q0 + q1;
     int cs = c0 + c1;
     __syncthreads();
-    sums_upto<ST>(qs, cs, wide, narrow);
+    sums_upto<ST>(qs, cs, wide_m, narrow);
     __syncthreads();
-    raw[b0] = qs - q0 - q1;
-    raw[b0 + 1] = qs - q1;
+    leave(b0, qs - (q0 + q1));
+    leave(b0 + 1, qs - q1);
     start[b0] = cs - c0 - c1;
     start[b0 + 1] = cs - c1;
     __syncthreads();
-    const int used = slots * cut;
     double ex[2], in[2];
     int c_in[2], c_ex[2];
     bool is[2];
@@ -926,9 +940,8 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       c_ex[e] = c_in[e] = 0;
       if (is[e]) {
         const int z = b / cut * cut, j = b / cut;
-        const u64 q = raw[b] - (whole ? 0ull : raw[z]);
-        ex[e] = (whole ? 0.0 : slot_m[j]) + (double)q * (1.0 / FINE_ONE);
-        in[e] = (whole ? 0.0 : slot_m[j]) + (double)(q + (e ? q1 : q0)) * (1.0 / FINE_ONE);
+        ex[e] = whole ? mass_at(b) : slot_m[j] + (mass_at(b) - mass_at(z));
+        in[e] = ex[e] + (e ? q1 : q0);
         c_ex[e] = whole ? start[b] : slot_c[j] + start[b] - start[z];
         c_in[e] = c_ex[e] + (e ? c1 : c0);
       }
@@ -936,7 +949,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       front_c[b] = c_ex[e];
     }
     if (whole) {
-      if (tid == ST - 1) masses = (double)qs * (1.0 / FINE_ONE);
+      if (tid == ST - 1) masses = qs;
       __syncthreads();
       mass = masses;
     }
@@ -1008,26 +1021,24 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   sort_down(v, raw, size);
   // mass up to and with each token, and its rank
   const int e0 = 2 * tid;
-  u64 q[2] = {0ull, 0ull};
   double w[2] = {0.0, 0.0}, in[2] = {0.0, 0.0};
   int rank[2] = {1 << 30, 1 << 30}, bin[2] = {0, 0};
 #pragma unroll
   for (int e = 0; e < 2; ++e)
     if (e0 + e < n) {
       w[e] = token_weight(v[e0 + e]);
-      q[e] = fine_of(w[e]);
       bin[e] = place(v[e0 + e]);
       if (e0 + e == 0 || place(v[e0 + e - 1]) != bin[e]) start[bin[e]] = e0 + e;
     }
-  const u64 sum = sum_upto<ST>(q[0] + q[1], wide);
-  raw[e0] = sum - q[1];
-  raw[e0 + 1] = sum;
+  const double sum = sum_upto<ST>(w[0] + w[1], wide_m);
+  leave(e0, sum - w[1]);
+  leave(e0 + 1, sum);
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < 2; ++e)
     if (e0 + e < n) {
       const int at = start[bin[e]];
-      in[e] = front_m[bin[e]] + (double)(raw[e0 + e] - (at > 0 ? raw[at - 1] : 0ull)) * (1.0 / FINE_ONE);
+      in[e] = front_m[bin[e]] + (mass_at(e0 + e) - (at > 0 ? mass_at(at - 1) : 0.0));
       rank[e] = front_c[bin[e]] + e0 + e - at;
     }
   // the ends: what is kept is the first `count`, of mass `mass`
@@ -1059,7 +1070,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   if (count < 1) { count = 1; mass = 1.0; }
   // the draw: the first over the goal, the last kept one where the sums' rounding leaves none
   const double goal = set.u * mass;
-  first_of(e0 < n && q[0] && rank[0] < count && in[0] > goal, e0 + 1 < n && q[1] && rank[1] < count && in[1] > goal, &got[2]);
+  first_of(e0 < n && w[0] > 0.0 && rank[0] < count && in[0] > goal, e0 + 1 < n && w[1] > 0.0 && rank[1] < count && in[1] > goal, &got[2]);
   __syncthreads();
   int at = got[2];
   if (at >= CAP) {
@@ -1067,7 +1078,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (e0 + e < n && q[e] && rank[e] < count) atomicMax(&got[3], e0 + e);
+      if (e0 + e < n && w[e] > 0.0 && rank[e] < count) atomicMax(&got[3], e0 + e);
     __syncthreads();
     at = max(got[3], 0);
   }
