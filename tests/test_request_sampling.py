@@ -240,9 +240,9 @@ def test_draws_from_equal_logits_far_below_one(V, down):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("V,n,settings", [(1000, 999, ((0, 0.0), (1000, 0.0), (0, 1e-12))), (40000, 900, ((901, 0.0), (901, 1e-12)))])
+@pytest.mark.parametrize("V,n,settings", [(1000, 999, ((0, 0.0), (1000, 0.0), (0, 1e-12))), (40000, 900, ((901, 0.0), (901, 1e-12))), (40000, 1500, ((0, 0.0), (1501, 0.0), (0, 1e-12)))])
 def test_draws_from_few_logits_far_below_one(V, n, settings):
-    """the same among tokens that are all put in order, at every u that is in the tail"""
+    """the same among tokens that are put in order, at every u that is in the tail"""
     x, u = [], []
     for i in range(0, 300, 1 if V < 2000 else 4):
         down = float(np.float32(21 + 0.01 * i))
@@ -256,3 +256,41 @@ def test_draws_from_few_logits_far_below_one(V, n, settings):
     x, r = torch.stack(x), len(u)
     for k, m in settings:
         check_finely(x, u, [1.0] * r, [k] * r, [1.0] * r, [m] * r)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [600, 1025, 8193, 20000, 40000, 128256])
+def test_equal_logits_among_masked_ones(V):
+    """n tokens of one value and nothing else: every share is a whole number of n-ths, and a p or u that is one too ends at the token that 64 bits end at"""
+    g = torch.Generator().manual_seed(V)
+    x, u, t, p = [], [], [], []
+    for n in (2, 3, 4, 8, 100):
+        for value, temperature in ((3.0, 1.0), (7.0, 0.7), (5.1, 1.0), (-2.3, 0.9)):
+            row = torch.full((V,), -INF)
+            row[torch.randperm(V, generator=g)[:n]] = value
+            for share in (0.25, 0.5, 0.75):
+                for uu, pp in ((share, 1.0), (0.6, share), (share, share)):
+                    x.append(row), u.append(uu), t.append(temperature), p.append(pp)
+    r = len(x)
+    check(torch.stack(x), u, t, [0] * r, p, [0.0] * r)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [1025, 40000, 128256])
+@pytest.mark.parametrize("k", [0, 2, 100, 1000, 1025])
+@pytest.mark.parametrize("rest,down", [(1000, 30.0), (1000, 25.0), (1 << 20, 34.0), (1 << 20, 60.0)])
+def test_equal_logits_above_a_faint_tail(V, rest, down, k):
+    """two and four largest, and tokens so far below that all of them together weigh some 1e-10 of the row: enough to say on which side of p the largest stand
+    (60 down: too little even for 64 bits, whose sums are whole)"""
+    g = torch.Generator().manual_seed(V)
+    x, u, t, p = [], [], [], []
+    for n in (2, 4):
+        for value, temperature in ((3.0, 1.0), (7.0, 0.7), (5.1, 1.0), (-2.3, 0.9)):
+            row = torch.full((V,), -INF)
+            order = torch.randperm(V, generator=g)
+            row[order[n:n + rest]] = value - down * temperature
+            row[order[:n]] = value
+            for share in (0.25, 0.5, 0.75):
+                x.append(row), u.append(0.6), t.append(temperature), p.append(share)
+    r = len(x)
+    check(torch.stack(x), u, t, [k] * r, p, [0.0] * r)

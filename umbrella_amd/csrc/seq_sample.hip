@@ -4,22 +4,24 @@
 // in front of which less than p of the first k's mass stands; those with w >= m.  The shortest prefix is kept, and of it the first token whose mass,
 // with all in front of it, exceeds u times the kept mass is drawn.
 //
-// Weights are 64-bit floats, summed as whole numbers: such sums are the same in any order, and a border between two tokens falls where a 64-bit sum of
-// any order puts it but for some 1e-12 of the mass.  (In 32 bits a flat row of 128256 values has thousands of borders that the sum's order moves.)
+// Weights are 64-bit floats, and a border between two tokens falls where 64-bit sums put it.  (In 32 bits a flat row of 128256 values has thousands of borders that
+// the sum's order moves.)  What is summed in no fixed order is summed as whole numbers.  Sums that are no better than some 1e-12 of the row (bins) or lack its
+// faintest tokens say where a border may be, never where it is: where the token drawn is not the same for all that they may stand for, the row is searched whole.
 //
 // Nothing is sorted but what stands next to a border.  Three launches (two for rows of one slice):
-//   slices   a row in slices, each read once into registers: its largest, and counts and masses of bins T / 32 wide, 1024 below the largest (what is
-//            further down weighs less than 2^-46 of the row).  Bins lie on one lattice, floor(32 x / T), and masses are relative to their bin's middle, so
-//            that slices' add up as whole numbers, count and mass in one 64-bit atomic
+//   slices   a row in slices, each read once into registers: its largest, and counts and masses of bins T / 32 wide, 1024 below the largest (a token
+//            further down weighs less than 2^-46, all of them together up to 7e-9).  Bins lie on one lattice, floor(32 x / T), and masses are relative to their bin's
+//            middle, so that slices' add up as whole numbers, count and mass in one 64-bit atomic
 //   collect  the row's bins, summed up from the top, say which bins hold the k-th value, the ends of top-p and min-p and the token drawn (intervals, since
-//            the mass behind p and u is known to a bin only); their tokens are collected.  A row of a small k has counts alone, and
+//            the mass behind p and u is known to a bin only, and the bins' masses to BIN_OFF); their tokens are collected.  A row of a small k has counts alone, and
 //            all tokens down to the k-th value's bin are collected
-//   resolve  a row's collected tokens by one workgroup: where they are many, bins again, up to 256 in each bin; then in order: the exact ends, then the draw
+//   resolve  a row's collected tokens by one workgroup: where they are many, bins again, up to 256 in each bin; then in order: the exact ends, then the draw, each by
+//            the least and the most that the sums in front may be
 // us (slices, collect, resolve): a row of 32000 3.8, 8, 9.9; 8 of 128256 5.2, 11.3, 10.2; 48 of 151936 12.2, 19.6, 16.6; 256 of 128256 37.4, 29.4, 14.
 // Bound by the logits where rows are many: the first launch reads them from memory, the second once more, from the cache behind it; by launches and barriers where
 // they are few.
 // Rows of up to SMALL_V values are taken whole by the last launch alone (1000 values 15 - 17 us, 1500 20 against 16 - 18 by two).  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
-// the thousand), is searched eight bits of the key at a time, by one workgroup, four passes a border (ms: 128256 equal values 1.1, 2.0 with a p, 2.9 with a k too; 48 rows
+// the thousand), or whose border the bins' masses leave open (by their bounds one of 500 000 nearly flat rows of 151936 with a p; two equal logits that p halves), is searched eight bits of the key at a time, by one workgroup, four passes a border (ms: 128256 equal values 1.1, 2.0 with a p, 2.9 with a k too; 48 rows
 // of as many rounded to whole numbers, with a p, 1.25).
 #include "seq_common.h"
 #include <algorithm>
@@ -215,18 +217,21 @@ __device__ __attribute__((noinline)) void sample_slow(int r, int* __restrict__ t
 // ------------------------------------------------------------------ bins
 constexpr int BINS = 1024, SMALL_V = 1024, CAP = 2048, K_COUNT = 1024, P_MAX = 64, FEW = 128;
 constexpr double PER_T = 32.0, LATTICE = 1099511627776.0;         // bins a T; beyond 2^40 neighbouring floats are 2^16 bins apart and more
-constexpr double BIN_ONE = 4294967296.0;                         // a bin's masses, in 2^-32 of its middle's weight: 48 bits for 2^15 of them, 16 above for their number
+// A bin's masses: 48 bits for 2^15 of them, 16 above for their number.  What each has above a bin's least weight, at most 0.0313 of its middle's, in 2^-37 of that:
+// half a step, 3.7e-12 of the least weight, and the polynomial's 5e-13 are BIN_OFF.  (The weights themselves would be held in 2^-32: 1.2e-10.)
+constexpr double BIN_ONE = 137438953472.0, BIN_LEAST = 0.9844964370058922, BIN_OFF = 4.5e-12;
+constexpr double FAINT = 1.4e-14;                                // more than a token below the bins weighs: e^(-1023 / 32)
 // resolve's bins: in 2^-46 of a power of two that a bin's weights reach to half of at least, so that 2^17 of them are good to 2^-46 of what they weigh, however far down
 constexpr int FINE_BITS = 46;
 __device__ __forceinline__ int fine_shift(int bin) { return (max(bin - 1, 0) * 47273) >> 20; }            // log2 of e^((bin - 1) / 32), rounded down
 __device__ __forceinline__ double power_of_two(int e) { return __longlong_as_double((long long)(1023 + e) << 52); }
 
-// e^((f - 1/2) / 32) of 0 <= f < 1 in whole numbers of 1 / BIN_ONE: the polynomial of degree 4 that meets it in the five Chebyshev points, good to 5e-13 of it,
-// rounded by the addition of 2^52.  The coefficients are held in registers: as literals each costs two moves an element.
+// e^((f - 1/2) / 32) - BIN_LEAST of 0 <= f < 1 in whole numbers of 1 / BIN_ONE: the polynomial of degree 4 that meets the first in the five Chebyshev points, good to 5e-13 of it,
+// without its constant, rounded by the addition of 2^52.  The coefficients are held in registers: as literals each costs two moves an element.
 struct BinExp {
   double c[5];
   __device__ __forceinline__ BinExp() {
-    const double k[5] = {0.9844964370058922, 0.03076551363223118, 0.0004807113442785956, 5.006866963355461e-06, 3.97368340715931e-08};
+    const double k[5] = {0.0, 0.03076551363223118, 0.0004807113442785956, 5.006866963355461e-06, 3.97368340715931e-08};
 #pragma unroll
     for (int i = 0; i < 5; ++i) c[i] = k[i] * BIN_ONE + (i == 0 ? MAGIC : 0.0);
 #pragma unroll
@@ -284,6 +289,10 @@ __device__ __forceinline__ float least_at(double goal, double per) {
 }
 
 struct SliceHead { float top; int at, pad[2]; };
+// how far off a bin's mass may be, of itself: and where a value lies on the lattice, of some |line| / T, is known to 2^-53 of that
+__device__ __forceinline__ double off_of(double line) { return BIN_OFF + 1e-17 * (fabs(line) + BINS); }
+// beside an infinite value, or one beyond the lattice, only its equals count
+__device__ __forceinline__ bool is_flat(float top, double per) { return top == INFINITY || !(fabs((double)top * per) < LATTICE); }
 // what collect leaves for resolve; `mass` and `count`: in front of each bin
 struct RowSaid {
   double all;
@@ -548,16 +557,17 @@ __global__ __launch_bounds__(BINS, NE > 16 ? 4 : 8) void sample_collect_kernel(c
         q += v[i] & 0xffffffffffffull;
       }
     }
-  // a bin's middle beside the largest; beside an infinite one, or one beyond the lattice, only its equals count
-  const bool flat = top == INFINITY || !(fabs((double)top * per) < LATTICE);
-  double m = flat ? (b == 0 ? (double)c : 0.0) : (double)q * (1.0 / BIN_ONE) * exp_down((first - b + 0.5 - line) * (1.0 / PER_T));
+  // (a bin's middle beside the largest)
+  const bool flat = is_flat(top, per);
+  double m = flat ? (b == 0 ? (double)c : 0.0) : fma((double)c, BIN_LEAST, (double)q * (1.0 / BIN_ONE)) * exp_down((first - b + 0.5 - line) * (1.0 / PER_T));
   const int c_own = c;
   sums_upto<NT>(c, m, wave_c, wave_m);
   c_in[b] = c;
   m_in[b] = m;
   __syncthreads();
   const int c_all = c_in[BINS - 1];
-  const double all = m_in[BINS - 1], slack = 1e-11 * all, m_ex = b > 0 ? m_in[b - 1] : 0.0;
+  // slack: both sides of a comparison may be off, here and where resolve makes it again; faint: what the tokens in no bin may weigh
+  const double all = m_in[BINS - 1], slack = (flat ? 1e-13 : 6.0 * off_of(line)) * all, faint = flat ? 0.0 : FAINT * (V - c_all), m_ex = b > 0 ? m_in[b - 1] : 0.0;
   // the bins that each end may lie in: k0, [p0, p1], [m0, m1], [d0, d1]; BINS: nowhere
   const int k = set.m > 1.0 ? 1 : set.k;
   const bool whole = top_k && top_k[r] >= 1 && top_k[r] <= K_COUNT, k_binds = k < c_all;
@@ -566,7 +576,7 @@ __global__ __launch_bounds__(BINS, NE > 16 ? 4 : 8) void sample_collect_kernel(c
   bool p_binds = false, m_binds = false;
   int m0 = BINS, m1 = BINS, from[4] = {0, BINS, BINS, BINS}, to[4] = {min(k0, BINS - 1), -1, -1, -1};       // runs of bins that are wanted
   if (!whole) {
-    const double mk_hi = k_binds ? m_in[k0] : all, mk_lo = !k_binds || k_exact ? mk_hi : k0 > 0 ? m_in[k0 - 1] : 0.0;
+    const double mk_hi = k_binds ? m_in[k0] : all + faint, mk_lo = !k_binds ? all : k_exact ? mk_hi : k0 > 0 ? m_in[k0 - 1] : 0.0;
     int p0 = BINS, p1 = BINS;
     if (set.p < 1.0) {
       const Two n = how_many(m < set.p * mk_lo - slack, m_ex < set.p * mk_hi + slack, &cells[1]);
@@ -736,9 +746,9 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   __shared__ short slot[BINS];
   __shared__ unsigned char want[CAP];
   __shared__ SlowRoom room;
-  __shared__ int from[P_MAX + 1], got[4], ranks, taken, sum_c;
+  __shared__ int from[P_MAX + 1], got[6], ranks, taken, sum_c;
   __shared__ Mass sum_m;
-  __shared__ double masses;
+  __shared__ double masses, masses_off;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* row = logits + (long)r * ld;
   const RowSettings set = row_settings(r, V, temperature, top_k, top_p, min_p, uniforms);
@@ -784,7 +794,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     }
     return;
   }
-  const double inv_t = 1.0 / set.t, per = PER_T / set.t, first = floor(line_of(top, per)), slack_of = 1e-11;
+  const double inv_t = 1.0 / set.t, per = PER_T / set.t, line = line_of(top, per), first = floor(line);
   auto value = [](u64 t) { return of_key((unsigned)(t >> 32)); };
   auto token_weight = [&](u64 t) { return (unsigned)(t >> 32) > KEY_NONE ? weight_at(value(t), top, inv_t) : 0.0; };
   int n = V, slots = 1;
@@ -854,7 +864,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       for (int e = 0; e < 4; ++e) if (i0 + e * ST < found) f(i0 + e * ST, t[e]);
     }
   };
-  if (tid < 4) got[tid] = CAP;
+  if (tid < 6) got[tid] = CAP;
   if (tid < 3) cells[tid] = 0;
   if (tid == 0) { taken = 0; sum_c = 0; sum_m = Mass{0ull, 0ll}; }
   if (many) for (int i = tid; i < CAP; i += ST) { raw[i] = 0ull; start[i] = 0; }
@@ -887,7 +897,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     }
     for (int i = tid; i < n; i += ST) enough(v[i], token_weight(v[i]));
   }
-  double end_m = 0.0;
+  double end_m = 0.0, front_of_m = 0.0;
   if (m_binds) {
     if (__ballot(count_m > 0)) {
 #pragma unroll
@@ -900,7 +910,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     __syncthreads();
     count_m = sum_c;
     end_m = sum_m.value();
-    if (!SMALL && !whole) { count_m += s.sums->count[m0]; end_m += s.sums->mass[m0]; }
+    if (!SMALL && !whole) { count_m += s.sums->count[m0]; front_of_m = s.sums->mass[m0]; end_m += front_of_m; }
   }
   __syncthreads();
   int how_k = SMALL || whole ? (k < n ? 1 : 0) : said.k_binds, count = SMALL || whole ? n : said.count_all;
@@ -912,6 +922,10 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       mass = said.k0 + 1 < BINS ? s.sums->mass[said.k0 + 1] : said.all;
     }
   }
+  // Sums from the bins: in front of a collected token, and of everything, off by `off` of them.  The collected tokens' own sums are good to 64 bits (bins of them to
+  // 2^-46 of each weight: 1e-14).  Of the first k, those that are in no bin may weigh `faint`.
+  const bool rough = !SMALL && !whole, flat = is_flat(top, per);
+  const double off = rough ? (flat ? 0.0 : off_of(line)) + 2e-14 : 0.0, faint = !SMALL && how_k == 0 && !flat ? FAINT * max(0, k - said.count_all) : 0.0;
   if (many) {
     // each bin's sums, from those in front of it; then which bins the ends may lie in, as collect does
     const int b0 = 2 * tid;
@@ -953,12 +967,12 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       __syncthreads();
       mass = masses;
     }
-    const double slack = slack_of * mass;
+    const double slack = (6.0 * off + 1e-12) * mass;
     auto before = [&](bool a0, bool a1, bool b0, bool b1, int call) -> Two {       // bins, of both a thread's
       return how_many(is[0] && a0, is[0] && b0, &cells[call], is[1] && a1, is[1] && b1);
     };
     const int k0 = how_k == 1 ? before(c_in[0] < k, c_in[1] < k, false, false, 0).a : used;
-    double lo = mass, hi = mass;
+    double lo = mass, hi = mass + faint;
     if (k0 < used) {
       __syncthreads();
 #pragma unroll
@@ -1041,44 +1055,62 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       in[e] = front_m[bin[e]] + (mass_at(e0 + e) - (at > 0 ? mass_at(at - 1) : 0.0));
       rank[e] = front_c[bin[e]] + e0 + e - at;
     }
-  // the ends: what is kept is the first `count`, of mass `mass`
+  // the ends: what is kept is the first `count`, whose mass is from mass - less to mass + more
   if ((SMALL || whole) && !many) {
     if (e0 <= n - 1 && n - 1 <= e0 + 1) masses = in[n - 1 - e0];
     __syncthreads();
     mass = masses;
   }
+  double in_off[2] = {0.0, 0.0}, less = off * mass, more = less + faint;
+  if (rough)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) if (e0 + e < n) in_off[e] = off * front_m[bin[e]] + 2e-14 * in[e];
   __syncthreads();
   if (how_k == 1) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) if (rank[e] == k - 1) { got[0] = 0; masses = in[e]; }
+    for (int e = 0; e < 2; ++e) if (rank[e] == k - 1) { got[0] = 0; masses = in[e]; masses_off = in_off[e]; }
   }
   __syncthreads();
-  if (how_k == 1 && got[0] == 0) { count = k; mass = masses; }
-  const double limit = fmax(set.p, 0.0) * mass;
+  if (how_k == 1 && got[0] == 0) { count = k; mass = masses; less = more = masses_off; }
   auto first_of = [&](bool x, bool y, int* to) {             // (one atomic a wave)
     const unsigned long long one = __ballot(x || y);
     if (one && lane == __ffsll(one) - 1) atomicMin(to, x ? e0 : e0 + 1);
   };
-  first_of(e0 < n && p_binds && in[0] >= limit, e0 + 1 < n && p_binds && in[1] >= limit, &got[1]);
+  // top-p's end: the first token that may reach p of the mass, and the first that does in any case
+  const double p = fmax(set.p, 0.0), limit = p * (mass - less), at_most = p * (mass + more);
+  first_of(e0 < n && p_binds && in[0] + in_off[0] >= limit, e0 + 1 < n && p_binds && in[1] + in_off[1] >= limit, &got[1]);
+  if (!SMALL) first_of(e0 < n && p_binds && in[0] - in_off[0] >= at_most, e0 + 1 < n && p_binds && in[1] - in_off[1] >= at_most, &got[4]);
   __syncthreads();
   const int kp = got[1];
+  bool open = false;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) if (e0 + e == kp) { ranks = rank[e] + 1; masses = in[e]; }
+  for (int e = 0; e < 2; ++e) if (e0 + e == kp) { ranks = rank[e] + 1; masses = in[e]; masses_off = in_off[e]; }
   __syncthreads();
-  if (m_binds && count_m < count) { count = count_m; mass = end_m; }
-  if (p_binds && kp < CAP && ranks < count) { count = ranks; mass = masses; }
-  if (count < 1) { count = 1; mass = 1.0; }
+  if (m_binds && count_m < count) { count = count_m; mass = end_m; less = more = rough ? off * front_of_m + 2e-14 * end_m : 0.0; }
+  if (p_binds && kp < CAP && ranks < count) {
+    count = ranks;
+    mass = masses;
+    less = more = masses_off;
+    open = !SMALL && got[4] != kp;
+  }
+  if (count < 1) { count = 1; mass = 1.0; less = more = 0.0; }
   // the draw: the first over the goal, the last kept one where the sums' rounding leaves none
-  const double goal = set.u * mass;
-  first_of(e0 < n && w[0] > 0.0 && rank[0] < count && in[0] > goal, e0 + 1 < n && w[1] > 0.0 && rank[1] < count && in[1] > goal, &got[2]);
+  const double goal = set.u * (mass - less), goal_most = set.u * (mass + more);
+  const bool kept[2] = {e0 < n && w[0] > 0.0 && rank[0] < count, e0 + 1 < n && w[1] > 0.0 && rank[1] < count};
+  first_of(kept[0] && in[0] + in_off[0] > goal, kept[1] && in[1] + in_off[1] > goal, &got[2]);
+  if (!SMALL) first_of(kept[0] && in[0] - in_off[0] > goal_most, kept[1] && in[1] - in_off[1] > goal_most, &got[5]);
   __syncthreads();
   int at = got[2];
+  if (!SMALL && (open || got[5] != at)) {
+    sample_slow(r, tokens, probs, row, V, set, top, room);
+    return;
+  }
   if (at >= CAP) {
     if (tid == 0) got[3] = -1;
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (e0 + e < n && w[e] > 0.0 && rank[e] < count) atomicMax(&got[3], e0 + e);
+      if (kept[e]) atomicMax(&got[3], e0 + e);
     __syncthreads();
     at = max(got[3], 0);
   }
