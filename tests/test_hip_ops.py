@@ -1019,3 +1019,25 @@ def test_h2d_layer_event_ordered(dev):
     torch.cuda.synchronize()
     assert torch.equal(out.cpu(), host)
     assert lib.umb_h2d_layer(None, C.c_void_p(host.data_ptr()), C.c_size_t(n), C.c_void_p(side.cuda_stream), None, None) == -22
+
+
+@pytest.mark.parametrize("V,k", [(96, 32), (96, 60), (96, 96), (12, 8), (13, 8), (4, 2), (512, 200), (800, 256), (4000, 1024)])
+def test_topk_of_vocabularies_of_a_few_k(dev, V, k):
+    """fewer than k threads have a value of the row: all its values are candidates.  Shares: 2^-24 for each of an exponent of at most 8 (its argument's rounding),
+    exp's own 2 steps and 10 additions, twice over (the share's sum): below 4e-6"""
+    from umbrella_amd import _lib
+    logits = torch.randn(3, V, generator=torch.Generator().manual_seed(V)).clamp(-4, 4)
+    tv, _ = logits.topk(k, dim=-1)
+    if k <= 64:
+        idx, val = torch.empty(3, k, dtype=torch.int32, device=dev), torch.empty(3, k, dtype=torch.float32, device=dev)
+        _lib.call("umb_topk_rows", idx, val, logits.to(dev), 3, V, k, None, None, None, None)
+        assert torch.equal(val.cpu(), tv) and torch.equal(logits.gather(1, idx.cpu().long()), tv)
+    seed, n = torch.tensor([5], dtype=torch.int64, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    for call in (_lib.call, _lib.seq_call):
+        got, di = torch.empty(3, dtype=torch.int32, device=dev), torch.empty(3, k, dtype=torch.int32, device=dev)
+        dp = torch.empty(3, k, dtype=torch.float32, device=dev)
+        call("umb_sample_rows", got, logits.to(dev), 3, V, n, n, 1.0, 1.0, k, 1.0, seed, k, di, dp)
+        assert torch.equal(logits.gather(1, di.cpu().long()), tv)
+        want = torch.softmax(tv.double(), -1)
+        assert bool(((dp.cpu().double() - want).abs() <= 4e-6 * want).all())
+        assert all(int(got[r]) in di[r].tolist() for r in range(3))

@@ -107,7 +107,8 @@ __device__ __forceinline__ int topk_select(const float* __restrict__ row, int V,
   const unsigned long long thr = thr_s;
   if ((V & 3) == 0) {
     const f32x4* r4 = reinterpret_cast<const f32x4*>(row);
-    const float thr_v = key_val(thr);                       // cheap float pre-filter, exact key compare after
+    // cheap float pre-filter, exact key compare after (fewer than k threads have a value, V < 4 k: no threshold, every value is a candidate)
+    const float thr_v = thr ? key_val(thr) : -INFINITY;
     for (int i = threadIdx.x; i < (V >> 2); i += 4 * 1024) {
       f32x4 q[4];
 #pragma unroll
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(1024) void sample_rows_kernel(float* __restrict__ l
   __syncthreads();
   if (keep) atomicAdd(&kc_s, 1);
   __syncthreads();
-  const int kc = kc_s;                                        // kept entries are a prefix of the sorted list
+  const int kc = max(kc_s, 1);                                // kept entries are a prefix of the sorted list (none: a row of NaN)
   const float kept_mass = cum[kc - 1];
   const unsigned long long r = mix64(mix64(*seed ^ ((unsigned long long)(unsigned)n << 32)) + blockIdx.x);
   const float u = (float)(r >> 40) * (1.0f / 16777216.0f);    // [0,1)
