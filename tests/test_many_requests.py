@@ -270,6 +270,18 @@ def test_the_engine_admits_what_fits_and_refuses_the_rest():
         e.step()
 
 
+@pytest.mark.gpu
+def test_continuations_differ_under_a_penalty_too():
+    """the engine's own sampling with a repetition penalty: every continuation draws for itself, the first as if it were alone, and a seed draws the same again"""
+    m = build("gitopel", "mixed", batch=4)
+    kw = dict(repetition_penalty=1.2, temperature=1.5, topk=60, topp=1.0, seed=3)
+    out = engine(m, **kw).generate_batch([[1, 2, 3]], 12, n=4)[0]
+    assert [len(t) for t in out] == [12] * 4 and len(set(map(tuple, out))) == 4
+    assert engine(m, **kw).generate_batch([[1, 2, 3]], 12, n=4)[0] == out
+    assert engine(m, **kw).generate_batch([[1, 2, 3]], 12)[0] == out[0]
+    assert engine(m, **{**kw, "seed": 4}).generate_batch([[1, 2, 3]], 12, n=4)[0] != out
+
+
 def test_forks_and_pages_on_the_host(monkeypatch):
     """the bookkeeping alone: random forks, extensions and closings, every page held as often as it is listed"""
     from umbrella_amd.attn import cache as C

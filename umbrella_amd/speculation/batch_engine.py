@@ -66,6 +66,7 @@ class Request:
     sampling: Sampling | None = None    # None: the engine's
     rng: random.Random | None = None
     nth: int = 0                        # which continuation of its prompt
+    seed: torch.Tensor | None = None    # of a further continuation's draws where the engine's generator makes them row by row
     adapter: int | None = None          # one of the model's
     copies: list = field(default_factory=list)       # further continuations of the same prompt
 
@@ -172,6 +173,15 @@ class BatchEngine(BaseEngine):
                 raise RuntimeError(f"request {r.id!r}: its logits leave no token to draw")
         return tokens
 
+    def _seed(self, r):
+        """What a request's row is drawn from by itself: that generator goes by seed, history length and row, and the continuations of a prompt have all three in
+        common, so that the further ones bring seeds of their own."""
+        if r.nth == 0:
+            return self.rng_state
+        if r.seed is None:
+            r.seed = send(torch.tensor([random.Random(f"{self.seed}/{r.id}").getrandbits(63)], dtype=torch.int64), self.device)
+        return r.seed
+
     def _sample(self, logits, reqs):
         """one token per logits row (row i belongs to reqs[i]) -> list of ints"""
         if any(r.sampling is not None for r in reqs):
@@ -188,7 +198,7 @@ class BatchEngine(BaseEngine):
                     slot = self.target_model.kv_cache.slot(r.id)
                     _lib.seq_call("umb_sample_rows", out[i:i + 1], logits[i:i + 1], 1, self.vocab_size, self.history[slot],
                                   self.hist_len[slot:slot + 1], float(self.repetition_penalty), float(self.temperature), k,
-                                  float(self.topp), self.rng_state, 0, None, None)
+                                  float(self.topp), self._seed(r), 0, None, None)
             else:
                 _lib.seq_call("umb_sample_rows", out, logits, R, self.vocab_size, self.history[0], self.step_count, 1.0,
                               float(self.temperature), k, float(self.topp), self.rng_state, 0, None, None)
