@@ -282,6 +282,30 @@ def test_continuations_differ_under_a_penalty_too():
     assert engine(m, **{**kw, "seed": 4}).generate_batch([[1, 2, 3]], 12, n=4)[0] != out
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(temperature=0.0), dict(temperature=1.3, topk=20, topp=0.95), dict(temperature=1.3, topk=20, repetition_penalty=1.3)])
+@pytest.mark.parametrize("place", [0, 1])
+def test_requests_without_settings_do_not_feel_their_neighbours(kw, place):
+    """what the engine's settings draw is the same beside requests with settings of their own, while they run and when they have ended"""
+    from umbrella_amd.speculation.batch_engine import Sampling
+    m = build("gitopel", "mixed", batch=4)
+
+    def texts(sampling):
+        e = engine(m, **kw)
+        e.repetition_penalty, penalty = 1.0, e.repetition_penalty          # (a request with settings is taken while the engine has no penalty)
+        each = [([1, 2, 3], 14, None), ([7, 8], 5, sampling), ([5, 4, 9, 9], 9, None)]
+        each.insert(2 * place, each.pop(1))
+        ids = [e.submit(p, n, sampling=s) for p, n, s in each]
+        e.repetition_penalty = penalty
+        while e.step():
+            pass
+        out = {tuple(p): e.finished[i].generated for (p, _, _), i in zip(each, ids)}
+        assert [len(out[tuple(p)]) for p, n, _ in each] == [n for _, n, _ in each]
+        return out
+    without, beside = texts(None), texts(Sampling(0.7, 5, 0.9, 0.1, seed=2))
+    assert all(without[p] == beside[p] for p in ((1, 2, 3), (5, 4, 9, 9)))
+
+
 def test_forks_and_pages_on_the_host(monkeypatch):
     """the bookkeeping alone: random forks, extensions and closings, every page held as often as it is listed"""
     from umbrella_amd.attn import cache as C

@@ -14,8 +14,8 @@ tokens (trace replay): it owns the page / slot bookkeeping and calls the model's
 It keeps the engine surface (speculation/base.py) so the front-ends work unchanged: ``prefill`` / ``append`` /
 ``speculative_decoding`` drive one conversation (a tree of size one: ``build_tree`` has nothing to build, ``verify`` is a
 plain decode step), ``generate`` / ``generate_stream`` answer one API request, ``generate_batch`` many.
-Sampling uses the same device kernels as the speculation engines (arg-max, or penalty / top-k / temperature / top-p) where the engine's
-settings hold for all; a request may bring its own (``Sampling``: temperature, top-k, top-p, min-p, seed), ask for several continuations of
+Sampling uses the same device kernels as the speculation engines (arg-max, or penalty / top-k / temperature / top-p) for requests that go by
+the engine's settings; a request may bring its own (``Sampling``: temperature, top-k, top-p, min-p, seed), ask for several continuations of
 its prompt (prefilled once, then forked: they share its full cache pages) and name a low-rank adapter of the model.
 """
 from __future__ import annotations
@@ -153,11 +153,13 @@ class BatchEngine(BaseEngine):
     def _greedy(self):
         return self.temperature < 0.05 and not (self.repetition_penalty > 1.01)
 
+    def _draws(self):
+        """whether the engine's kernels take the engine's settings"""
+        return self._greedy() or (1 <= min(int(self.topk), self.vocab_size) <= 1024 and self.topp > 0)
+
     def _sample_own(self, logits, reqs):
-        """each row by its request's settings, or by the engine's where it has none, from its own random numbers"""
+        """each row by its request's settings, or by the engine's where it has none, from its own random numbers -> int32 tokens on the device"""
         R = len(reqs)
-        if any(r.sampling is None for r in reqs) and self.repetition_penalty > 1.01:
-            raise ValueError("a repetition penalty does not go with requests that have settings of their own in the batch")
         mine = [r.sampling or Sampling(0.0 if self.temperature < 0.05 else self.temperature, int(self.topk), float(self.topp)) for r in reqs]
         for r in reqs:
             if r.rng is None:
@@ -166,12 +168,7 @@ class BatchEngine(BaseEngine):
         host = torch.tensor([[s.temperature for s in mine], [s.top_p for s in mine], [s.min_p for s in mine], [r.rng.random() for r in reqs]], dtype=torch.float32)
         both = send(torch.cat([host.view(torch.int32), torch.tensor([[s.top_k for s in mine]], dtype=torch.int32)]), self.device)
         f = both.view(torch.float32)
-        tokens, _ = sample_rows(logits[:R], f[3], temperature=f[0], top_k=both[4], top_p=f[1], min_p=f[2])
-        tokens = tokens.tolist()
-        for r, t in zip(reqs, tokens):
-            if t < 0:
-                raise RuntimeError(f"request {r.id!r}: its logits leave no token to draw")
-        return tokens
+        return sample_rows(logits[:R], f[3], temperature=f[0], top_k=both[4], top_p=f[1], min_p=f[2])[0]
 
     def _seed(self, r):
         """What a request's row is drawn from by itself: that generator goes by seed, history length and row, and the continuations of a prompt have all three in
@@ -183,9 +180,22 @@ class BatchEngine(BaseEngine):
         return r.seed
 
     def _sample(self, logits, reqs):
-        """one token per logits row (row i belongs to reqs[i]) -> list of ints"""
-        if any(r.sampling is not None for r in reqs):
-            return self._sample_own(logits, reqs)
+        """one token per logits row (row i belongs to reqs[i]) -> list of ints.  Rows without settings of their own are drawn as they would be if no row had any."""
+        rows = [i for i, r in enumerate(reqs) if r.sampling is None]
+        if len(rows) == len(reqs):
+            return self._sample_engine(logits, reqs, rows).tolist()
+        tokens = self._sample_own(logits, reqs)
+        if rows and (self._draws() or self.repetition_penalty > 1.01):
+            at = send(torch.tensor(rows, dtype=torch.long), tokens.device)
+            tokens[at] = self._sample_engine(logits, reqs, rows)[at]
+        tokens = tokens.tolist()
+        for r, t in zip(reqs, tokens):
+            if r.sampling is not None and t < 0:
+                raise RuntimeError(f"request {r.id!r}: its logits leave no token to draw")
+        return tokens
+
+    def _sample_engine(self, logits, reqs, rows):
+        """`rows` of the logits by the engine's settings, kernels and generator, which goes by the place of a row -> int32 tokens on the device, others' as well"""
         R = logits.shape[0]
         out = self.sampled[:R]
         if self._greedy():
@@ -194,15 +204,18 @@ class BatchEngine(BaseEngine):
             k = min(int(self.topk), self.vocab_size)
             self.step_count += 1
             if self.repetition_penalty > 1.01:
-                for i, r in enumerate(reqs):          # every request is penalised over its own history
+                for i in rows:                        # every request is penalised over its own history
+                    r = reqs[i]
                     slot = self.target_model.kv_cache.slot(r.id)
                     _lib.seq_call("umb_sample_rows", out[i:i + 1], logits[i:i + 1], 1, self.vocab_size, self.history[slot],
                                   self.hist_len[slot:slot + 1], float(self.repetition_penalty), float(self.temperature), k,
                                   float(self.topp), self._seed(r), 0, None, None)
             else:
+                if len(rows) < R:                     # (the others' are not its business: a row of its own in their places)
+                    logits = logits[send(torch.tensor([i if r.sampling is None else rows[0] for i, r in enumerate(reqs)], dtype=torch.long), logits.device)]
                 _lib.seq_call("umb_sample_rows", out, logits, R, self.vocab_size, self.history[0], self.step_count, 1.0,
                               float(self.temperature), k, float(self.topp), self.rng_state, 0, None, None)
-        return out.tolist()
+        return out
 
     def _record(self, req, tokens):
         """append tokens to the request's device-side history (read by the repetition penalty)"""
