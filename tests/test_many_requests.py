@@ -306,6 +306,68 @@ def test_requests_without_settings_do_not_feel_their_neighbours(kw, place):
     assert all(without[p] == beside[p] for p in ((1, 2, 3), (5, 4, 9, 9)))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("step", [0, 1, 4])
+@pytest.mark.parametrize("copies", [1, 2])
+def test_a_request_without_a_token_ends_alone(step, copies, monkeypatch):
+    """one request's logits are NaN in a step: it ends there with an error, and its neighbours draw what they draw beside one that ends there by itself"""
+    from umbrella_amd.speculation.batch_engine import RequestError, Sampling
+    m = build("gitopel", "mixed", batch=8)
+
+    def texts(bad):
+        e = engine(m, temperature=1.2, topk=20)
+        inner, calls = e.run_step, [0]
+
+        def run_step(entries, end=()):
+            logits = inner(entries, end)
+            if bad and calls[0] == step:
+                for i, (rid, _, _) in enumerate(entries):
+                    if rid in ("bad", ("bad", 1)):
+                        logits[i] = float("nan")
+            calls[0] += 1
+            return logits
+        monkeypatch.setattr(e, "run_step", run_step)
+        own = Sampling(0.9, 30, 0.9, 0.01, seed=4)
+        e.submit([1, 2, 3], 9, request_id="own", sampling=own)
+        e.submit([8, 8], 9 if bad else step + 1, request_id="bad", sampling=own, n=copies)
+        e.submit([4, 5, 6, 7], 11, request_id="engine's")
+        while e.step():
+            pass
+        assert not m.kv_cache.seqs and not any(m.kv_cache.refs) and not e.running
+        return e.finished
+    got, want = texts(True), texts(False)
+    for i in ("own", "engine's"):
+        assert got[i].generated == want[i].generated and got[i].error is None
+    for i in ["bad", ("bad", 1)][:copies]:
+        assert got[i].error and got[i].generated == want[i].generated[:step]
+    e = engine(m)
+    monkeypatch.setattr(e, "run_step", lambda entries, inner=e.run_step: inner(entries) * float("nan"))
+    with pytest.raises(RequestError) as err:
+        e.generate_batch([[1, 2], [3]], 4, sampling=Sampling())
+    assert err.value.outputs == [[], []] and not e.finished and not m.kv_cache.seqs
+
+
+@pytest.mark.gpu
+def test_settings_that_cannot_be_drawn_by_are_refused_before_a_step():
+    from umbrella_amd._lib import UmbError
+    m = build("gitopel", "mixed", batch=4)
+    e, want = engine(m, temperature=1.0, topk=20), engine(m, temperature=1.0, topk=20).generate_batch([[1, 2, 3], [4]], 6)
+    ids = [e.submit([1, 2, 3], 6), e.submit([4], 6)]
+    for wrong in (0, 3):                                      # before the prompts, and in mid-text
+        for _ in range(wrong):
+            e.step()
+        for name, value in (("topk", 0), ("topk", 2000), ("topp", 0.0)):
+            good = getattr(e, name)
+            setattr(e, name, value)
+            if value != 2000:                                 # (more than the vocabulary: all of it)
+                with pytest.raises(UmbError):
+                    e.step()
+            setattr(e, name, good)
+    while e.step():
+        pass
+    assert [e.finished[i].generated for i in ids] == want
+
+
 def test_forks_and_pages_on_the_host(monkeypatch):
     """the bookkeeping alone: random forks, extensions and closings, every page held as often as it is listed"""
     from umbrella_amd.attn import cache as C

@@ -54,6 +54,13 @@ class Sampling:
             raise ValueError(f"a temperature of 0 and more, top_p and min_p of 0 to 1 and a top_k of 0 (all) and more are wanted, got {self}")
 
 
+class RequestError(RuntimeError):
+    """some of a call's requests ended without what they were asked for; ``outputs``: what every one of the call has generated"""
+    def __init__(self, failed, outputs):
+        super().__init__("; ".join(f"request {r.id!r}: {r.error}" for r in failed))
+        self.outputs = outputs
+
+
 @dataclass
 class Request:
     id: object
@@ -61,6 +68,7 @@ class Request:
     max_new_tokens: int
     generated: list = field(default_factory=list)
     done: bool = False
+    error: str | None = None            # why it ended before its time
     pending: int | None = None          # sampled, not yet fed through the model
     recorded: int = 0                   # tokens written to the device-side history of its slot
     sampling: Sampling | None = None    # None: the engine's
@@ -180,7 +188,8 @@ class BatchEngine(BaseEngine):
         return r.seed
 
     def _sample(self, logits, reqs):
-        """one token per logits row (row i belongs to reqs[i]) -> list of ints.  Rows without settings of their own are drawn as they would be if no row had any."""
+        """One token per logits row (row i belongs to reqs[i]) -> list of ints; -1 for a row with settings of its own that leaves no token.  Rows without settings are
+        drawn as they would be if no row had any."""
         rows = [i for i, r in enumerate(reqs) if r.sampling is None]
         if len(rows) == len(reqs):
             return self._sample_engine(logits, reqs, rows).tolist()
@@ -188,11 +197,7 @@ class BatchEngine(BaseEngine):
         if rows and (self._draws() or self.repetition_penalty > 1.01):
             at = send(torch.tensor(rows, dtype=torch.long), tokens.device)
             tokens[at] = self._sample_engine(logits, reqs, rows)[at]
-        tokens = tokens.tolist()
-        for r, t in zip(reqs, tokens):
-            if r.sampling is not None and t < 0:
-                raise RuntimeError(f"request {r.id!r}: its logits leave no token to draw")
-        return tokens
+        return tokens.tolist()
 
     def _sample_engine(self, logits, reqs, rows):
         """`rows` of the logits by the engine's settings, kernels and generator, which goes by the place of a row -> int32 tokens on the device, others' as well"""
@@ -287,10 +292,17 @@ class BatchEngine(BaseEngine):
     def step(self) -> bool:
         """One scheduler step (prefill of a fresh batch, or one decoded token for every running request).  Returns
         whether anything is left to do."""
-        if not self.running:
+        fresh = not self.running
+        if fresh:
             self._admit()
             if not self.running:
                 return False
+        if not self._draws() and any(r.sampling is None for r in self.running) and (self.repetition_penalty > 1.01 or all(r.sampling is None for r in self.running)):
+            if fresh:                           # (before the model has seen anything: the step can be made again with other settings)
+                self.queue.extendleft(reversed(self.running))
+                self.running.clear()
+            raise _lib.UmbError(f"the engine's settings cannot be drawn by: top-k {self.topk} (1 to 1024 is wanted), top-p {self.topp} (above 0)")
+        if fresh:
             batch = list(self.running)
             entries = [(r.id, r.prompt, [len(r.prompt) - 1]) for r in batch]
             for r in batch:
@@ -308,6 +320,10 @@ class BatchEngine(BaseEngine):
         new = self._sample(logits, batch)
         end = []
         for r, tok in zip(batch, new):
+            if tok < 0:                         # (its neighbours' tokens hold, and the model has taken in what they were drawn behind)
+                r.error = "its logits leave no token to draw"
+                end.append(r)
+                continue
             r.generated.append(tok)
             r.pending = tok
             self._record(r, [tok])
@@ -334,7 +350,8 @@ class BatchEngine(BaseEngine):
     @torch.inference_mode()
     def generate_batch(self, prompts, max_new_tokens: int = 128, sampling=None, n: int = 1, adapters=None):
         """prompts: list of token-id lists -> list of generated token-id lists (greedy or sampled per the engine's knobs).  sampling: one
-        ``Sampling`` for all, or one (or None) per prompt; adapters: a number (or None) per prompt; n > 1: a list of n continuations per prompt."""
+        ``Sampling`` for all, or one (or None) per prompt; adapters: a number (or None) per prompt; n > 1: a list of n continuations per prompt.
+        RequestError, once all have ended, if some did so before their time."""
         each = list(sampling) if isinstance(sampling, (list, tuple)) else [sampling] * len(prompts)
         named = list(adapters) if adapters is not None else [None] * len(prompts)
         if len(each) != len(prompts) or len(named) != len(prompts):
@@ -342,9 +359,12 @@ class BatchEngine(BaseEngine):
         ids = [self.submit(p, max_new_tokens, sampling=s, n=n, adapter=a) for p, s, a in zip(prompts, each, named)]
         while self.step():
             pass
-        if n == 1:
-            return [self.finished.pop(i).generated for i in ids]
-        return [[self.finished.pop(i if k == 0 else (i, k)).generated for k in range(n)] for i in ids]
+        done = [[self.finished.pop(i if k == 0 else (i, k)) for k in range(n)] for i in ids]
+        out = [[r.generated for r in each] if n > 1 else each[0].generated for each in done]
+        failed = [r for each in done for r in each if r.error]
+        if failed:
+            raise RequestError(failed, out)
+        return out
 
     # ------------------------------------------------------------------ one conversation (engine surface)
     def prefill(self, text: str):
@@ -488,6 +508,8 @@ class BatchEngine(BaseEngine):
             text = " ".join(self._decode_words(r.generated))
             yield text, "Output Tokens {} | TPOT {:.2f} ms ".format(len(r.generated), 1000 * (time.time() - t1) / len(r.generated))
         r = self.finished.pop(rid)
+        if r.error:
+            raise RequestError([r], [r.generated])
         yield " ".join(self._decode_words(r.generated)), "Output Tokens {} | TPOT {:.2f} ms ".format(
             len(r.generated), 1000 * (time.time() - t1) / max(len(r.generated), 1))
 
