@@ -368,6 +368,38 @@ def test_settings_that_cannot_be_drawn_by_are_refused_before_a_step():
     assert [e.finished[i].generated for i in ids] == want
 
 
+@pytest.mark.gpu
+def test_a_request_that_does_not_fit_stands_in_nobodys_way():
+    m = build("gitopel", "mixed", batch=4, max_length=60, max_tokens=64)
+    want = engine(m).generate_batch([[4, 5]], 5)[0]
+    for holds, bad in (([1, 2], dict(input_ids=[1, 2, 3], max_new_tokens=5, n=4)),               # three slots are left
+                       (tokens(60, 96, 1), dict(input_ids=[1, 2, 3], max_new_tokens=50, n=1)),   # too few pages
+                       (tokens(60, 96, 1), dict(input_ids=[1, 2, 3], max_new_tokens=20, n=3))):
+        e = engine(m)
+        m.open("holder")
+        last_logits(m, "holder", holds)
+        wrong, right = e.submit(**bad), e.submit([4, 5], 5)
+        with pytest.raises(RuntimeError):
+            e.step()
+        while e.step():
+            pass
+        assert e.finished[right].generated == want and not e.queue
+        for i in [wrong] + [(wrong, k) for k in range(1, bad["n"])]:
+            assert e.finished[i].error and not e.finished[i].generated
+        m.close("holder")
+        assert not m.kv_cache.seqs
+    # a single request waits for a slot
+    for s in "abcd":
+        m.open(s)
+    e = engine(m)
+    i = e.submit([4, 5], 5)
+    assert not e.step() and list(e.queue)
+    m.close("b")
+    while e.step():
+        pass
+    assert e.finished[i].generated == want
+
+
 def test_forks_and_pages_on_the_host(monkeypatch):
     """the bookkeeping alone: random forks, extensions and closings, every page held as often as it is listed"""
     from umbrella_amd.attn import cache as C

@@ -266,22 +266,29 @@ class BatchEngine(BaseEngine):
         return whole + len(r.copies) * (whole - shared)
 
     def _admit(self):
-        """static batching: called only when nothing runs; first come first served while slots and pages last"""
+        """static batching: called only when nothing runs; first come first served while slots and pages last.  RuntimeError for a request that does not fit
+        though nothing runs: it ends there, and those behind it are admitted by the next step."""
         cache = self.target_model.kv_cache
-        budget = len(cache.free_pages)
-        slots = 0
-        while self.queue and slots + len(self.queue[0].copies) < min(self.max_batch, len(cache.free_slots)):
+        budget, room, slots = len(cache.free_pages), min(self.max_batch, len(cache.free_slots)), 0
+        while self.queue:
             r = self.queue[0]
-            need = self._pages_wanted(r)
-            if need > budget:
-                if not self.running:
-                    raise RuntimeError(f"request {r.id!r} needs {need} cache pages, the cache has {budget} free")
+            need, seqs = self._pages_wanted(r), 1 + len(r.copies)
+            if slots + seqs > room or need > budget:
                 break
             budget -= need
-            slots += 1 + len(r.copies)
+            slots += seqs
             self.running.append(self.queue.popleft())
-        if not self.running and self.queue and self.queue[0].copies:
-            raise RuntimeError(f"request {self.queue[0].id!r} needs {1 + len(self.queue[0].copies)} sequence slots, {len(cache.free_slots)} are free")
+        if self.running or not self.queue or (seqs > room and seqs == 1):     # (no slot at all: others hold them, and it waits)
+            return
+        why = f"needs {seqs} sequence slots, {room} are free" if seqs > room else f"needs {need} cache pages, the cache has {budget} free"
+        self._fail(self.queue.popleft(), why)
+        raise RuntimeError(f"request {r.id!r} {why}")
+
+    def _fail(self, r, why):
+        for q in (r, *r.copies):
+            q.error, q.done = why, True
+            self.finished[q.id] = q
+        r.copies = []
 
     def _retire(self, r):
         r.done = True
