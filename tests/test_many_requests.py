@@ -400,6 +400,32 @@ def test_a_request_that_does_not_fit_stands_in_nobodys_way():
     assert e.finished[i].generated == want
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("after", [0, 1, 2])
+def test_queued_requests_do_not_run_with_adapters_that_they_did_not_name(after):
+    """adapters loaded anew, fewer or as many, while a request that names one is queued: it ends with an error, the others run"""
+    m = build("tutunex", "mixed", batch=4)
+    V, e = m.config.vocab_size, engine(m)
+    want = engine(m).generate_batch([tokens(4, V, 1)], 5)[0]
+    m.load_adapters(adapters_for(m, 5))
+    first, named, last = e.submit(tokens(4, V, 1), 5), e.submit(tokens(4, V, 1), 5, n=2, adapter=1), e.submit(tokens(4, V, 1), 5)
+    m.load_adapters(adapters_for(m, 6)[:after])
+    while e.step():
+        pass
+    assert e.finished[first].generated == e.finished[last].generated == want
+    for i in (named, (named, 1)):
+        assert e.finished[i].error and not e.finished[i].generated
+    assert not m.kv_cache.seqs and not e.queue
+    if after:
+        e.submit(tokens(4, V, 1), 5, request_id="new", adapter=after - 1)
+        while e.step():
+            pass
+        assert len(e.finished["new"].generated) == 5
+        e.submit(tokens(4, V, 1), 5, request_id="alone", adapter=0)
+        m.load_adapters([])
+        assert not e.step() and e.finished["alone"].error
+
+
 def test_forks_and_pages_on_the_host(monkeypatch):
     """the bookkeeping alone: random forks, extensions and closings, every page held as often as it is listed"""
     from umbrella_amd.attn import cache as C

@@ -479,7 +479,7 @@ class SeqMixLM(LLMBase):
         return self._bufs["logits"]
 
     # ------------------------------------------------------------------ adapters
-    n_adapters = 0
+    n_adapters = adapters_loaded = 0         # how many there are, and how often they have been loaded
 
     def load_adapters(self, adapters):
         """Low-rank adapters that sequences may name (``open(seq_id, adapter=i)``), beside the layers' input and output products.  adapters: one dict
@@ -510,6 +510,7 @@ class SeqMixLM(LLMBase):
             if set(a) - known:
                 raise ValueError(f"adapter {n}: no such product: {sorted(set(a) - known, key=str)}")
         self.n_adapters, self._adapter_stacks, self._adapter_structs = S, stacks, structs
+        self.adapters_loaded += 1
 
     def _adapter_struct(self, ids_ptr: int, T: int):
         """the step's adapters, and the scratch that has to live until its launches are made"""

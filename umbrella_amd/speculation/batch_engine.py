@@ -76,6 +76,7 @@ class Request:
     nth: int = 0                        # which continuation of its prompt
     seed: torch.Tensor | None = None    # of a further continuation's draws where the engine's generator makes them row by row
     adapter: int | None = None          # one of the model's
+    loaded: int = 0                     # the model's load_adapters that it counts by
     copies: list = field(default_factory=list)       # further continuations of the same prompt
 
 
@@ -236,7 +237,8 @@ class BatchEngine(BaseEngine):
     # ------------------------------------------------------------------ scheduler
     def submit(self, input_ids, max_new_tokens: int = 128, request_id=None, sampling: Sampling | None = None, n: int = 1, adapter: int | None = None):
         """Queues a request.  n > 1: so many continuations of the prompt; the further ones are requests (request_id, 1) to (request_id, n - 1) of
-        their own, each with random numbers of its own."""
+        their own, each with random numbers of its own.  adapter: one of those that the model has now; if others are loaded before the request runs,
+        it ends with an error."""
         ids = [int(t) for t in (input_ids.reshape(-1).tolist() if isinstance(input_ids, torch.Tensor) else input_ids)]
         if not ids:
             raise ValueError("a request needs at least one prompt token")
@@ -254,7 +256,7 @@ class BatchEngine(BaseEngine):
             raise ValueError(f"the model has {getattr(self.target_model, 'n_adapters', 0)} adapters, got number {adapter}")
         if request_id is None:
             request_id, self._next_id = self._next_id, self._next_id + 1
-        r = Request(request_id, ids, int(max_new_tokens), sampling=sampling, adapter=adapter)
+        r = Request(request_id, ids, int(max_new_tokens), sampling=sampling, adapter=adapter, loaded=getattr(self.target_model, "adapters_loaded", 0))
         r.copies = [Request((request_id, i), ids, int(max_new_tokens), sampling=sampling, adapter=adapter, nth=i) for i in range(1, n)]
         self.queue.append(r)
         return request_id
@@ -272,6 +274,9 @@ class BatchEngine(BaseEngine):
         budget, room, slots = len(cache.free_pages), min(self.max_batch, len(cache.free_slots)), 0
         while self.queue:
             r = self.queue[0]
+            if r.adapter is not None and r.loaded != self.target_model.adapters_loaded:
+                self._fail(self.queue.popleft(), f"the model's adapters are others than those that number {r.adapter} was one of")
+                continue
             need, seqs = self._pages_wanted(r), 1 + len(r.copies)
             if slots + seqs > room or need > budget:
                 break
