@@ -426,6 +426,24 @@ def test_queued_requests_do_not_run_with_adapters_that_they_did_not_name(after):
         assert not e.step() and e.finished["alone"].error
 
 
+@pytest.mark.gpu
+def test_api_requests_with_min_p_are_answered_whatever_the_engine_runs_by():
+    m = build("gitopel", "mixed", batch=4)
+    ask = dict(input_ids=[1, 2, 3], max_new_tokens=8)
+    for kw in (dict(repetition_penalty=1.3, temperature=0.0), dict(repetition_penalty=1.3, temperature=1.2, topk=20), dict(temperature=0.0, topk=-1, topp=1.5)):
+        want = engine(m, **kw).generate(**ask)["generated_tokens"] if kw.get("topk", 1) > 0 else engine(m, temperature=0.0).generate(**ask)["generated_tokens"]
+        for min_p in (0.0, 0.1):
+            assert engine(m, **kw).generate(**ask, min_p=min_p)["generated_tokens"] == want
+        *_, (text, _) = engine(m, **kw).generate_stream(**ask, min_p=0.1)
+        assert text.split() == [str(t) for t in want]
+    # a top-p above 1 keeps all, as it does without min_p; settings that are none are refused still
+    e = engine(m, temperature=1.2, topk=0, topp=1.5)
+    assert e.generate(**ask, min_p=0.05, seed=3)["generated_tokens"] == e.generate(**ask, topp=1.0, min_p=0.05, seed=3)["generated_tokens"]
+    for bad in (dict(min_p=-0.1), dict(min_p=1.5), dict(min_p=float("nan")), dict(min_p=0.1, topk=-1)):
+        with pytest.raises(ValueError):
+            engine(m, temperature=1.2).generate(**ask, **bad)
+
+
 def test_forks_and_pages_on_the_host(monkeypatch):
     """the bookkeeping alone: random forks, extensions and closings, every page held as often as it is listed"""
     from umbrella_amd.attn import cache as C

@@ -469,11 +469,18 @@ class BatchEngine(BaseEngine):
         self.rng_state.fill_(seed)
 
     def _api_sampling(self, api_args):
-        """an API request that names min_p has settings of its own; others run by the engine's"""
-        if api_args.get("min_p") is None:
+        """An API request that names min_p has settings of its own, made of the engine's; others run by the engine's.  So does one that names it where own settings are
+        not possible (a repetition penalty, a vocabulary too large), as it would on the other engines, which do not know min_p."""
+        min_p, seed = api_args.get("min_p"), api_args.get("seed")
+        if min_p is None:
             return None
-        seed = api_args.get("seed")
-        return Sampling(0.0 if self.temperature < 0.05 else float(self.temperature), int(self.topk), float(self.topp), float(api_args["min_p"]), None if seed is None else int(seed))
+        if self.repetition_penalty > 1.01 or self.vocab_size > MAX_VOCAB:
+            logger.warning("min_p is not taken: " + ("it does not go with a repetition penalty" if self.repetition_penalty > 1.01 else f"the vocabulary has more than {MAX_VOCAB} tokens"))
+            return None
+        seed = None if seed is None else int(seed)
+        if self.temperature < 0.05:             # (greedy, whatever the rest says)
+            return Sampling(0.0, min_p=float(min_p), seed=seed)
+        return Sampling(float(self.temperature), int(self.topk), min(float(self.topp), 1.0), float(min_p), seed)
 
     def _request_ids(self, api_args):
         input_ids = api_args.get("input_ids", None)
