@@ -76,6 +76,16 @@ def test_ranks(name, R):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("T", [1, 40, 200, 300])
+def test_ranks_that_end_in_every_tile(name, T):
+    """Products of tiles of 16 ranks, of which some adapters have all, some a few of the last and some none: with a branch between two of them, the last sum of four was
+    read before it was there (rank 72: of 67 and 71)"""
+    for R in (32, 64, 128):
+        check(make(T, 264, 84, 8, R, TYPES[name], seed=T + R, ids="any", ranks=[R, R // 2 + 8, R // 2 + 1, R - 7, R - 15, 9, 24, R - 16]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("K,N", [(1, 1), (7, 5), (8, 4), (31, 66), (33, 255), (40, 256), (100, 257), (184, 520), (1000, 1030), (4096, 300), (264, 5000)])
 def test_widths(name, K, N):
     check(make(19, K, N, 3, 8, TYPES[name], seed=K, ids="any"))

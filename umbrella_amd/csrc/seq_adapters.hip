@@ -211,7 +211,8 @@ __device__ __forceinline__ void down_sums(f32x4 (&acc)[RF], char* stage, const i
     for (int i = 0; i < NA; ++i) *reinterpret_cast<u32x4*>(stage + (16 * TF + row + i * ROWS) * LD + piece * 16) = av[i];
     __syncthreads();
     if (k + AHEAD * KC < k1) load(xv, av, k + AHEAD * KC);
-    // (all ranks and rows, zeros among them: with a branch between two products the compiler leaves too few cycles in front of the first one's sums)
+    // (All ranks and rows, zeros among them.  With `if (16 * f < ra)` in front of a product the compiler, in the kernels of 8 tiles of ranks, moves the last of its four sums
+    // to another register one to three instructions behind it, where eight are wanted: 28 such moves, and none without it.)
     constexpr int MINE = TF == 4 ? D::STEPS : D::STEPS / 4;
 #pragma unroll
     for (int s0 = 0; s0 < MINE; ++s0) {
