@@ -746,7 +746,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   __shared__ short slot[BINS];
   __shared__ unsigned char want[CAP];
   __shared__ SlowRoom room;
-  __shared__ int from[P_MAX + 1], got[6], ranks, taken, sum_c;
+  __shared__ int from[P_MAX + 1], got[4], ranks, taken, sum_c;
   __shared__ Mass sum_m;
   __shared__ double masses, masses_off;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -864,7 +864,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
       for (int e = 0; e < 4; ++e) if (i0 + e * ST < found) f(i0 + e * ST, t[e]);
     }
   };
-  if (tid < 6) got[tid] = CAP;
+  if (tid < 4) got[tid] = 2 * CAP;
   if (tid < 3) cells[tid] = 0;
   if (tid == 0) { taken = 0; sum_c = 0; sum_m = Mass{0ull, 0ll}; }
   if (many) for (int i = tid; i < CAP; i += ST) { raw[i] = 0ull; start[i] = 0; }
@@ -985,7 +985,7 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
         lo = mass = hi;
       } else lo = front_m[k0];
       __syncthreads();
-      if (tid == 0) got[0] = CAP;
+      if (tid == 0) got[0] = 2 * CAP;
     }
     int p0 = used, p1 = -1;
     if (p_binds) {
@@ -1072,16 +1072,17 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
   }
   __syncthreads();
   if (how_k == 1 && got[0] == 0) { count = k; mass = masses; less = more = masses_off; }
-  auto first_of = [&](bool x, bool y, int* to) {             // (one atomic a wave)
+  // twice the first element for which it may be so, and 1 if it need not be (in any case it is so for no earlier one); one atomic a wave
+  auto first_of = [&](bool x, bool y, bool sure_x, bool sure_y, int* to) {
     const unsigned long long one = __ballot(x || y);
-    if (one && lane == __ffsll(one) - 1) atomicMin(to, x ? e0 : e0 + 1);
+    if (one && lane == __ffsll(one) - 1) atomicMin(to, x ? 2 * e0 + !sure_x : 2 * e0 + 2 + !sure_y);
   };
-  // top-p's end: the first token that may reach p of the mass, and the first that does in any case
+  // top-p's end: the first token that reaches p of the mass
   const double p = fmax(set.p, 0.0), limit = p * (mass - less), at_most = p * (mass + more);
-  first_of(e0 < n && p_binds && in[0] + in_off[0] >= limit, e0 + 1 < n && p_binds && in[1] + in_off[1] >= limit, &got[1]);
-  if (!SMALL) first_of(e0 < n && p_binds && in[0] - in_off[0] >= at_most, e0 + 1 < n && p_binds && in[1] - in_off[1] >= at_most, &got[4]);
+  first_of(e0 < n && p_binds && in[0] + in_off[0] >= limit, e0 + 1 < n && p_binds && in[1] + in_off[1] >= limit, in[0] - in_off[0] >= at_most, in[1] - in_off[1] >= at_most,
+           &got[1]);
   __syncthreads();
-  const int kp = got[1];
+  const int kp = got[1] >> 1;
   bool open = false;
 #pragma unroll
   for (int e = 0; e < 2; ++e) if (e0 + e == kp) { ranks = rank[e] + 1; masses = in[e]; masses_off = in_off[e]; }
@@ -1091,17 +1092,16 @@ __global__ __launch_bounds__(ST) void sample_resolve_kernel(int* __restrict__ to
     count = ranks;
     mass = masses;
     less = more = masses_off;
-    open = !SMALL && got[4] != kp;
+    open = !SMALL && (got[1] & 1);
   }
   if (count < 1) { count = 1; mass = 1.0; less = more = 0.0; }
   // the draw: the first over the goal, the last kept one where the sums' rounding leaves none
   const double goal = set.u * (mass - less), goal_most = set.u * (mass + more);
   const bool kept[2] = {e0 < n && w[0] > 0.0 && rank[0] < count, e0 + 1 < n && w[1] > 0.0 && rank[1] < count};
-  first_of(kept[0] && in[0] + in_off[0] > goal, kept[1] && in[1] + in_off[1] > goal, &got[2]);
-  if (!SMALL) first_of(kept[0] && in[0] - in_off[0] > goal_most, kept[1] && in[1] - in_off[1] > goal_most, &got[5]);
+  first_of(kept[0] && in[0] + in_off[0] > goal, kept[1] && in[1] + in_off[1] > goal, in[0] - in_off[0] > goal_most, in[1] - in_off[1] > goal_most, &got[2]);
   __syncthreads();
-  int at = got[2];
-  if (!SMALL && (open || got[5] != at)) {
+  int at = got[2] >> 1;
+  if (!SMALL && (open || (got[2] & 1))) {
     sample_slow(r, tokens, probs, row, V, set, top, room);
     return;
   }

@@ -74,7 +74,7 @@ class Request:
     sampling: Sampling | None = None    # None: the engine's
     rng: random.Random | None = None
     nth: int = 0                        # which continuation of its prompt
-    seed: torch.Tensor | None = None    # of a further continuation's draws where the engine's generator makes them row by row
+    seed: torch.Tensor | None = field(default=None, compare=False)        # of a further continuation's draws where the engine's generator makes them row by row
     adapter: int | None = None          # one of the model's
     loaded: int = 0                     # the model's load_adapters that it counts by
     copies: list = field(default_factory=list)       # further continuations of the same prompt
