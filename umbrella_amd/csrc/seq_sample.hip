@@ -17,7 +17,7 @@
 //            all tokens down to the k-th value's bin are collected
 //   resolve  a row's collected tokens by one workgroup: where they are many, bins again, up to 256 in each bin; then in order: the exact ends, then the draw, each by
 //            the least and the most that the sums in front may be
-// us (slices, collect, resolve): a row of 32000 3.8, 8, 9.9; 8 of 128256 5.2, 11.3, 10.2; 48 of 151936 12.2, 19.6, 16.6; 256 of 128256 37.4, 29.4, 14.
+// us (slices, collect, resolve): a row of 32000 3.8, 8, 10.4; 8 of 128256 5.2, 11.2, 10.4; 48 of 151936 12.6, 19.8, 17; 256 of 128256 37.7, 29.5, 14.6.
 // Bound by the logits where rows are many: the first launch reads them from memory, the second once more, from the cache behind it; by launches and barriers where
 // they are few.
 // Rows of up to SMALL_V values are taken whole by the last launch alone (1000 values 15 - 17 us, 1500 20 against 16 - 18 by two).  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
