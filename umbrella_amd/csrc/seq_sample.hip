@@ -20,9 +20,10 @@
 // us (slices, collect, resolve): a row of 32000 3.8, 8, 10.4; 8 of 128256 5.2, 11.2, 10.4; 48 of 151936 12.6, 19.8, 17; 256 of 128256 37.7, 29.5, 14.6.
 // Bound by the logits where rows are many: the first launch reads them from memory, the second once more, from the cache behind it; by launches and barriers where
 // they are few.
-// Rows of up to SMALL_V values are taken whole by the last launch alone (1000 values 15 - 17 us, 1500 20 against 16 - 18 by two).  A row with more than CAP tokens next to a border, or a quarter of a slice (equal logits by
-// the thousand), or whose border the bins' masses leave open (by their bounds one of 500 000 nearly flat rows of 151936 with a p; two equal logits that p halves), is searched eight bits of the key at a time, by one workgroup, four passes a border (ms: 128256 equal values 1.1, 2.0 with a p, 2.9 with a k too; 48 rows
-// of as many rounded to whole numbers, with a p, 1.25).
+// Rows of up to SMALL_V values are taken whole by the last launch alone (1000 values 15 - 17 us, 1500 20 against 16 - 18 by two).
+// Searched eight bits of the key at a time, by one workgroup, four passes a border: a row with more than CAP tokens next to a border, or a quarter of a slice (equal
+// logits by the thousand), or whose border the bins' masses leave open (by their bounds one of 500 000 nearly flat rows of 151936 with a p; two equal logits that p
+// halves).  ms: 128256 equal values 1.1, 2.0 with a p, 2.9 with a k too; 48 rows of as many rounded to whole numbers, with a p, 1.25.
 #include "seq_common.h"
 #include <algorithm>
 
